@@ -354,6 +354,84 @@ LBQ_API int lbq_q_push(const int8_t* q_codes, const float* q_scale, int rows_pad
 LBQ_API int lbq_peer_wait(const uint64_t* peers, int nranks, int rank, int64_t xchg_off, int signals,
                   uint64_t timeout_ns, void* stream);
 
+/* ---------------------------------------------------------------- paged 8-bit KV cache, rotary positions
+ * A cache that stays in 8 bits: the reference keeps bf16 K/V in one buffer a layer and quantizes its whole window
+ * again for every attention call (lingbot/layers/kv_cache.py:11-88, lingbot/layers/sage_preq.py:107-128); here a token
+ * is quantized once, when it is written, and sessions share, fork and drop pages through page tables. These entries
+ * have no counterpart in the reference.
+ *
+ * A page holds 64 tokens of every K/V head:
+ *   k_pages, v_pages  [num_pages][heads][64][128] codes, int8 (LBQ_PAGE_INT8) or e4m3 (LBQ_PAGE_E4M3), 128-byte aligned
+ *   k_amax, v_amax    f32 [num_pages][heads]: value = code * amax / 127 (int8) or / 448 (e4m3)
+ *   table             int32 [batch] rows of `width` page ids (row stride st_b; ids past a sequence's pages are not
+ *                     read): token t of sequence b is row t % 64 of page table[b][t / 64]
+ * num_pages * heads * 64 stays below 2^31. A page id outside the pool, or a length or start outside the table, is not
+ * followed: it sets the device status to 0x305 (the tokens count as masked, or are not written). */
+#define LBQ_PAGE_INT8 0
+#define LBQ_PAGE_E4M3 1
+
+/* Rotary positions: out of place or in place (y == x with equal strides), the first `rot` channels of every head of x
+ * [B, L, heads, dim] and, in the same launch, of x2 [B, L, heads2, dim] (null with heads2 = 0): (x0, x1) -> (x0 c -
+ * x1 s, x0 s + x1 c) for the pairs (2i, 2i + 1) (interleaved != 0) or (i, i + rot / 2). c, s: row pos of the f32 tables
+ * [rope_rows][rot / 2] (row stride rope_stride); pos [B, L] int32 or int64 (pos64; element strides sp_b, sp_l), or null
+ * for start + l. inverse != 0 turns back, which is also the gradient. dtype 0 bf16, 1 fp16, 2 fp32; dim even, at most
+ * 512; rot even. A position outside the tables sets the device status to 0x306 and leaves its token as it is.
+ * The reference ropes interleaved pairs by fp64 tables of the chunk's own tokens (transformer.py:134-146). */
+LBQ_API int lbq_rope(const void* x, int64_t sx_b, int64_t sx_l, int64_t sx_h, void* y, int64_t sy_b, int64_t sy_l,
+                     int64_t sy_h, int heads, const void* x2, int64_t sx2_b, int64_t sx2_l, int64_t sx2_h, void* y2,
+                     int64_t sy2_b, int64_t sy2_l, int64_t sy2_h, int heads2, int batch, int len, int dim,
+                     const float* rope_cos, const float* rope_sin, int64_t rope_stride, int64_t rope_rows, int rot,
+                     int interleaved, const void* pos, int pos64, int64_t sp_b, int64_t sp_l, int64_t start, int inverse,
+                     int dtype, void* stream);
+
+/* Quantizing write of new tokens k, v [B, L, heads, 128] (dtype bf16 or fp16) at tokens start[b] .. start[b] + lens[b]
+ * of each sequence (start null: start0 for all; lens null: L). For a page and head that new tokens x enter, a = max(amax
+ * of the tokens it holds before start, max finite |x|, 2^-40); its held codes become round(c * a_old / a), the new ones
+ * round(x * Q / a) (exact decisions; int8 half to even, e4m3 to nearest); infinities become +-Q and NaN 0. Rows at and
+ * past start that get no new token keep their codes. With rope tables (see lbq_rope; rot a multiple of 8, or of 16 for
+ * the half layout; 16-byte aligned, row stride a multiple of 4) K is rotated first, at pos or at its token index,
+ * with the bits that lbq_rope followed by the plain write gives. No two sequences of one call may share a page that
+ * they write. */
+LBQ_API int lbq_page_write(const void* k, int64_t sk_b, int64_t sk_l, int64_t sk_h, const void* v, int64_t sv_b,
+                           int64_t sv_l, int64_t sv_h, void* k_pages, float* k_amax, void* v_pages, float* v_amax,
+                           int64_t num_pages, int heads, int fmt, const int32_t* table, int64_t st_b, int width,
+                           const int32_t* start, int64_t start0, const int32_t* lens, int batch, int len,
+                           const float* rope_cos, const float* rope_sin, int64_t rope_stride, int64_t rope_rows, int rot,
+                           int interleaved, const void* pos, int pos64, int64_t sp_b, int64_t sp_l, int dtype,
+                           void* stream);
+
+/* Reads tokens start[b] .. start[b] + lens[b] of each sequence back as values k_out, v_out [B, L, heads, 128] (bf16 or
+ * fp16); rows past lens[b] become 0. */
+LBQ_API int lbq_page_read(const void* k_pages, const float* k_amax, const void* v_pages, const float* v_amax,
+                          int64_t num_pages, int heads, int fmt, const int32_t* table, int64_t st_b, int width,
+                          const int32_t* start, int64_t start0, const int32_t* lens, int batch, int len, void* k_out,
+                          int64_t sk_b, int64_t sk_l, int64_t sk_h, void* v_out, int64_t sv_b, int64_t sv_l,
+                          int64_t sv_h, int dtype, void* stream);
+
+/* Copies whole pages src[i] -> dst[i] (codes of all heads, both tensors, amax) in each of `layers` pools that lie
+ * layer_bytes (codes) and layer_amax (floats) apart. src and dst are host arrays, read before the call returns. No page
+ * may be written twice, nor both read and written. */
+LBQ_API int lbq_page_copy(void* k_pages, float* k_amax, void* v_pages, float* v_amax, int64_t num_pages, int heads,
+                          int layers, int64_t layer_bytes, int64_t layer_amax, const int32_t* src, const int32_t* dst,
+                          int pairs, void* stream);
+
+/* Key splits that lbq_paged_attn would use for these shapes, and the scratch bytes of a split count (0 for one). */
+LBQ_API int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t max_kv_len);
+LBQ_API size_t lbq_paged_attn_workspace(int batch, int q_len, int heads, int group, int num_splits);
+
+/* Attention of q [B, Lq, heads * group, 128] (bf16 or fp16; query head h uses K/V head h / group) over the cache:
+ * softmax(sm_scale q . k) v over the tokens j < kv_lens[b] (null: kv_len0 for all) and, with causal != 0, j <= kv_lens[b]
+ * - q_lens[b] + i for query token i (the queries are the sequence's last tokens). q_lens null: Lq. Codes and scales are
+ * used as they are; sums are fp32. Rows that see no token, and rows i >= q_lens[b], become 0 (lse -inf). out as q; lse
+ * null or f32 [B, Lq, heads * group], natural logarithm. sm_scale <= 0 means 1/sqrt(128). num_splits > 1 splits the
+ * keys; workspace as lbq_paged_attn_workspace says, not shared by calls that may overlap. */
+LBQ_API int lbq_paged_attn(const void* q, int64_t sq_b, int64_t sq_l, int64_t sq_h, const void* k_pages,
+                           const float* k_amax, const void* v_pages, const float* v_amax, int64_t num_pages, int heads,
+                           int fmt, const int32_t* table, int64_t st_b, int width, const int32_t* kv_lens,
+                           int64_t kv_len0, const int32_t* q_lens, int batch, int q_len, int group, int causal,
+                           float sm_scale, void* out, int64_t so_b, int64_t so_l, int64_t so_h, float* lse,
+                           int num_splits, void* workspace, size_t workspace_bytes, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,7 @@
 
 #include "../../include/lbq.h"
 #include "lbq_kernels.h"
+#include "lbq_paged.h"
 
 namespace {
 
@@ -105,6 +106,9 @@ int set_error(int code, const char* fmt, ...) {
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
   va_end(ap);
   return code;
+}
+int make_page_map(CUtensorMap* m, const void* base, uint64_t rows, const char* name, uint32_t box_rows) {
+  return make_map(m, base, 128, rows, 1, 128, rows * 128, name, box_rows);
 }
 }  // namespace lbq
 

@@ -58,6 +58,20 @@ SIGNATURES = {
     "lbq_attn_fwd_keys": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp,
                                  _vp, _i32, _i32, _i64, _i32, _i64, _i64, _vp]),
     "lbq_keys_combine": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _i64, _i64, _vp]),
+    "lbq_rope": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
+                        _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _i64, _i32, _i32, _vp, _i32, _i64, _i64, _i64,
+                        _i32, _i32, _vp]),
+    "lbq_page_write": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp,
+                              _i64, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i64, _i64, _i32, _i32, _vp, _i32,
+                              _i64, _i64, _i32, _vp]),
+    "lbq_page_read": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _i32, _vp,
+                             _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "lbq_page_copy": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _i64, _vp, _vp, _i32, _vp]),
+    "lbq_paged_attn_splits": (_i32, [_i32, _i32, _i32, _i32, _i64]),
+    "lbq_paged_attn_workspace": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "lbq_paged_attn": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _i64,
+                              _vp, _i32, _i32, _i32, _i32, _f32, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _sz, _i32,
+                              _vp]),
     "lbq_q_push": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i64, _i64, _vp, _i32, _i32, _i64, _i32, _vp]),
 }
 
@@ -97,6 +111,16 @@ def call(name, *args):
         msg = lib.lbq_last_error().decode(errors="replace")
         raise LbqError(f"{name} failed ({rc}): {msg}")
     return rc
+
+
+def call_on(device, name, *args):
+    """`call` with the current stream of `device` as the last argument, made with that device current."""
+    import torch
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call(name, *args, stream)
+    with torch.cuda.device(device):
+        return call(name, *args, stream)
 
 
 def device_status(clear=True):

@@ -1,0 +1,237 @@
+"""Paged cache and rotary: what is refused before any GPU work, and PagedCache's page bookkeeping against a model that
+keeps every session's tokens in a list."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+from lingbot_b200 import _lib, paged_cache, rope
+
+
+def test_pages_and_tables_are_checked():
+    z = torch.zeros
+    with pytest.raises(TypeError):
+        paged_cache.Pages(z(2, 1, 64, 128), z(2, 1, 64, 128), z(2, 1), z(2, 1))
+    i8 = torch.int8
+    with pytest.raises(ValueError, match="codes"):
+        paged_cache.Pages(z(2, 1, 32, 128, dtype=i8), z(2, 1, 32, 128, dtype=i8), z(2, 1), z(2, 1))
+    with pytest.raises(ValueError, match="CUDA"):
+        paged_cache.Pages(z(2, 1, 64, 128, dtype=i8), z(2, 1, 64, 128, dtype=i8), z(2, 1), z(2, 1))
+    with pytest.raises(TypeError, match="format"):
+        paged_cache.alloc_pages(1, 1, "cpu", torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        rope.tables(4, 8, device="cpu")
+    for bad in ({"type": "linear", "factor": 0.5}, {"type": "other", "factor": 2.0},
+                {"type": "banded", "factor": 2.0, "original": 10, "low": 4, "high": 4}):
+        with pytest.raises(ValueError):
+            rope.tables(4, 8, scaling=bad, device="cpu")
+    for rot in (0, 7):
+        with pytest.raises(ValueError, match="rot"):
+            rope.tables(4, rot, device="cpu")
+
+
+def _aligned(nbytes=4096):
+    buf = ctypes.create_string_buffer(nbytes + 256)
+    at = (ctypes.addressof(buf) + 255) // 256 * 256
+    return buf, at
+
+
+def test_c_entries_refuse_bad_arguments():
+    """Every call here is refused before a CUDA call is made."""
+    lib = _lib.load()
+    keep, p = _aligned()
+    err = lib.lbq_last_error
+
+    def read(**kw):
+        a = dict(kp=p, ka=p, vp=p, va=p, n=4, heads=1, fmt=0, table=p, st=4, width=4, start=None, s0=0, lens=None, b=1, l=8,
+                 ko=p, vo=p, s=(1024, 128, 128), dtype=0)
+        a.update(kw)
+        return lib.lbq_page_read(a["kp"], a["ka"], a["vp"], a["va"], a["n"], a["heads"], a["fmt"], a["table"], a["st"],
+                                 a["width"], a["start"], a["s0"], a["lens"], a["b"], a["l"], a["ko"], *a["s"], a["vo"],
+                                 *a["s"], a["dtype"], None)
+    for kw, rc, word in [(dict(kp=None), 1, b"null"), (dict(kp=p + 16), 2, b"aligned"), (dict(fmt=2), 1, b"fmt"),
+                         (dict(n=0), 1, b"pages"), (dict(n=1 << 25), 1, b"2^31"), (dict(heads=0), 1, b"heads"),
+                         (dict(table=None), 1, b"table"), (dict(width=0), 1, b"table"), (dict(b=0), 1, b"batch"),
+                         (dict(b=2, st=3), 1, b"table"), (dict(l=-1), 1, b"len"), (dict(dtype=2), 1, b"dtype"),
+                         (dict(s0=-1), 1, b"start"), (dict(s0=250), 1, b"outside"), (dict(ko=p + 2), 2, b"aligned"),
+                         (dict(s=(1024, 129, 128)), 2, b"strides")]:
+        assert read(**kw) == rc and word in err(), (kw, err())
+
+    def copy(pairs=(0,), to=(1,), n=4, layers=1, lb=0, la=0):
+        s, d = ((ctypes.c_int32 * len(x))(*x) for x in (pairs, to))
+        return lib.lbq_page_copy(p, p, p, p, n, 1, layers, lb, la, s, d, len(pairs), None)
+    assert copy(pairs=(4,)) == 1 and b"outside" in err()
+    assert copy(to=(-1,)) == 1 and b"outside" in err()
+    assert copy(layers=0) == 1
+    assert copy(layers=2, lb=4 * 8192 - 128, la=4) == 1 and b"layer" in err()
+    assert copy(pairs=(), to=()) == 0
+
+    def attn(**kw):
+        a = dict(q=p, out=p, table=p, width=4, kv=None, kv0=100, b=1, lq=1, group=1, splits=1, ws=None, wsb=0, heads=1)
+        a.update(kw)
+        return lib.lbq_paged_attn(a["q"], 1024, 128, 128, p, p, p, p, 4, a["heads"], 0, a["table"], 4, a["width"], a["kv"],
+                                  a["kv0"], None, a["b"], a["lq"], a["group"], 0, 0.0, a["out"], 1024, 128, 128, None,
+                                  a["splits"], a["ws"], a["wsb"], 0, None)
+    for kw, rc, word in [(dict(q=None), 1, b"null"), (dict(out=p + 8), 2, b"aligned"), (dict(kv0=257), 1, b"kv_len"),
+                         (dict(kv0=-1), 1, b"kv_len"), (dict(group=0), 1, b"group"), (dict(b=70000), 1, b"batch"),
+                         (dict(splits=2), 1, b"workspace"), (dict(splits=2, ws=p, wsb=8), 1, b"workspace"),
+                         (dict(lq=1 << 28, group=5), 1, b"large")]:
+        assert attn(**kw) == rc and word in err(), (kw, err())
+    assert attn(lq=0) == 0
+    assert lib.lbq_paged_attn_workspace(1, 1, 12, 1, 1) == 0
+    assert lib.lbq_paged_attn_workspace(1, 1, 12, 1, 4) >= 4 * 12 * 130 * 4
+    assert lib.lbq_paged_attn_splits(1, 1, 12, 1, 1) == 1
+    assert lib.lbq_paged_attn_splits(1, 1, 12, 1, 30160) > 1
+
+    def write(**kw):
+        a = dict(k=p, start=None, s0=0, l=8, cos=None, sin=None, rs=0, rr=0, rot=0, inter=1)
+        a.update(kw)
+        return lib.lbq_page_write(a["k"], 1024, 128, 128, p, 1024, 128, 128, p, p, p, p, 4, 1, 0, p, 4, 4, a["start"], a["s0"],
+                                  None, 1, a["l"], a["cos"], a["sin"], a["rs"], a["rr"], a["rot"], a["inter"], None, 0, 0, 0,
+                                  0, None)
+    for kw, rc, word in [(dict(k=None), 1, b"null"), (dict(s0=249), 1, b"outside"), (dict(cos=p), 1, b"rope"),
+                         (dict(cos=p, sin=p, rs=64, rr=4, rot=130), 1, b"rot"),
+                         (dict(cos=p, sin=p, rs=64, rr=0, rot=128), 1, b"rows"),
+                         (dict(cos=p, sin=p, rs=64, rr=4, rot=12), 2, b"rope"),
+                         (dict(cos=p, sin=p, rs=64, rr=4, rot=24, inter=0), 2, b"rope"),
+                         (dict(cos=p, sin=p, rs=66, rr=4, rot=128), 2, b"rope")]:
+        assert write(**kw) == rc and word in err(), (kw, err())
+
+    def turn(**kw):
+        a = dict(x=p, h=1, x2=None, h2=0, dim=128, rot=128, start=0, dtype=0, l=4)
+        a.update(kw)
+        return lib.lbq_rope(a["x"], 512, 128, 128, p, 512, 128, 128, a["h"], a["x2"], 0, 0, 0, None, 0, 0, 0, a["h2"], 1,
+                            a["l"], a["dim"], p, p, 64, 4, a["rot"], 1, None, 0, 0, 0, a["start"], 0, a["dtype"], None)
+    for kw, rc, word in [(dict(x=None), 1, b"null"), (dict(dtype=3), 1, b"dtype"), (dict(h=0), 1, b"heads"),
+                         (dict(x2=p), 1, b"x2"), (dict(dim=514), 1, b"dim"), (dict(rot=130), 1, b"rot"),
+                         (dict(rot=3), 1, b"rot"), (dict(start=-1), 1, b"start"), (dict(x=p + 1), 2, b"aligned")]:
+        assert turn(**kw) == rc and word in err(), (kw, err())
+    assert turn(l=0) == 0
+    del keep
+
+
+class Tokens:
+    """Stand-in pool on the CPU: one head; a token's code is its row of the pages."""
+
+    def __init__(self, monkeypatch, num_pages, layers=2):
+        monkeypatch.setattr(paged_cache.Pages, "__post_init__", lambda self: None)
+        monkeypatch.setattr(paged_cache.Pages, "layer", lambda self, i: self)
+        shape = (layers, num_pages, 1, 64, 128)
+        self.mem = torch.full((num_pages, 64), -1, dtype=torch.long)
+        self.cache = paged_cache.PagedCache(paged_cache.Pages(
+            torch.empty(shape, dtype=torch.int8), torch.empty(shape, dtype=torch.int8), torch.empty(shape[:3]),
+            torch.empty(shape[:3])), max_pages=8)
+        self.moves = []
+
+        def copy(pages, src, dst):
+            assert len(set(dst)) == len(dst) and not set(dst) & set(src)
+            self.moves += list(zip(src, dst))
+            self.mem[list(dst)] = self.mem[list(src)]
+        monkeypatch.setattr(paged_cache, "copy_pages", copy)
+
+    def write(self, plan, fresh):
+        for b, n in enumerate(plan.new):
+            for i in range(n):
+                t = int(plan.start[b]) + i
+                self.mem[int(plan.table[b, t // 64]), t % 64] = fresh[b][i]
+
+    def read(self, s):
+        ids, n = self.cache.page_ids(s), self.cache.tokens(s)
+        return [int(self.mem[ids[t // 64], t % 64]) for t in range(n)]
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_bookkeeping_keeps_every_sessions_tokens(monkeypatch, seed):
+    r = random.Random(seed)
+    pool = Tokens(monkeypatch, 40)
+    c, model, stamp = pool.cache, {}, 0
+    for _ in range(300):
+        what = r.choice(["open", "step", "step", "step", "fork", "close", "evict", "compact"])
+        some = list(model)
+        if what == "open" and len(model) < 6:
+            model[c.open()] = []
+        elif what == "step" and some:
+            chosen = r.sample(some, r.randint(1, len(some)))
+            new = [r.choice([0, 1, r.randint(1, 90)]) for _ in chosen]
+            before = (c.free_pages, {s: c.page_ids(s) for s in some})
+            try:
+                plan = c.plan(chosen, new)
+            except (RuntimeError, ValueError):
+                assert before == (c.free_pages, {s: c.page_ids(s) for s in some})
+                continue
+            fresh = [[(stamp := stamp + 1) for _ in range(n)] for n in new]
+            pool.write(plan, [[-7] * n for n in new])               # a pass that the next one replaces
+            pool.write(plan, fresh)
+            if r.random() < 0.8:
+                c.commit(plan)
+                for s, f in zip(chosen, fresh):
+                    model[s] = model[s] + f
+        elif what == "fork" and some and len(model) < 6:
+            s = r.choice(some)
+            model[c.fork(s)] = list(model[s])
+        elif what == "close" and some:
+            s = r.choice(some)
+            c.close(s)
+            del model[s]
+        elif what == "evict" and some:
+            s = r.choice(some)
+            n = len(model[s]) // 64
+            sink = r.randint(0, n) * 64
+            out = r.randint(0, n - sink // 64) * 64
+            c.evict(s, sink, out)
+            model[s] = model[s][:sink] + model[s][sink + out:]
+        elif what == "compact":
+            c.compact()
+            used = {p for s in model for p in c.page_ids(s)}
+            assert not used or max(used) < len(used)
+        for s in model:
+            assert pool.read(s) == model[s] and c.tokens(s) == len(model[s])
+        used = [p for s in model for p in c.page_ids(s)]
+        assert len(set(used)) + c.free_pages == c.num_pages
+
+
+def test_stale_plans_and_bad_calls_are_refused(monkeypatch):
+    pool = Tokens(monkeypatch, 12)
+    c = pool.cache
+    a = c.open()
+    c.commit(c.plan([a], 70))
+    plan = c.plan([a], 5)
+    b = c.fork(a)
+    for call in (lambda: c.commit(plan), lambda: c.attend(0, plan, None), lambda: c.write(0, plan, None, None)):
+        with pytest.raises(RuntimeError, match="plan again"):
+            call()
+    plan = c.plan([a, b], [3, 4])                                   # both write the shared unfinished page
+    assert len(pool.moves) == 1 and c.page_ids(a)[1] != c.page_ids(b)[1] and c.page_ids(a)[0] == c.page_ids(b)[0]
+    c.commit(plan)
+    with pytest.raises(RuntimeError, match="moved on"):
+        c.commit(plan)
+    with pytest.raises(ValueError, match="twice"):
+        c.plan([a, a], 1)
+    with pytest.raises(KeyError):
+        c.plan([99], 1)
+    with pytest.raises(ValueError, match="exceed"):
+        c.plan([a], 8 * 64)
+    with pytest.raises(ValueError, match="multiples"):
+        c.evict(a, 0, 10)
+    with pytest.raises(ValueError, match="fewer"):
+        c.evict(a, 64, 64)
+    with pytest.raises(ValueError, match="negative"):
+        c.plan([a], [-1])
+    old = c.plan([b], 1)
+    c.evict(b, 0, 64)
+    with pytest.raises(RuntimeError, match="plan again"):
+        c.commit(old)
+    fixed = c.fixed_plan(1)
+    table = fixed.table
+    got = c.plan([b], 60, into=fixed)
+    assert got is fixed and fixed.table is table and int(fixed.kv_lens[0]) == c.tokens(b) + 60
+    with pytest.raises(ValueError, match="cannot take"):
+        c.plan([a, b], 1, into=fixed)
+
+
+def test_copy_pages_refuses_overlap():
+    for src, dst, word in [([1, 2], [3], "source"), ([1, 2], [3, 3], "twice"), ([1, 2], [2, 3], "both")]:
+        with pytest.raises(ValueError, match=word):
+            paged_cache.copy_pages(None, src, dst)
+    paged_cache.copy_pages(None, [], [])

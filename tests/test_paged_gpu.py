@@ -1,0 +1,413 @@
+"""The paged 8-bit cache on the GPU against tests/_paged.py in float64: written codes and scales bit for bit, read-back
+values within the output's rounding, attention within the tolerance derived in _paged.attend plus half a step of the
+output type."""
+import pytest
+import torch
+
+from tests import _paged as P
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = pytest.mark.parametrize("fmt", [torch.int8, torch.float8_e4m3fn], ids=["int8", "e4m3"])
+TYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+
+
+def pool(pages):
+    from lingbot_b200 import paged_cache
+    return paged_cache.Pages(*(t.cuda() for t in pages))
+
+
+def raw(t):
+    return t.cpu().view(torch.uint8)
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------------------------------------ write and window
+@FORMATS
+@TYPES
+@pytest.mark.parametrize("heads,length,starts,lens", [
+    (3, 1, [0, 63, 64, 130], None), (2, 64, [0, 64], None), (1, 200, [5, 0, 127], [200, 1, 77]),
+    (2, 130, [190, 64], [0, 130]), (12, 7, [60], None)])
+def test_write_gives_the_exact_codes(fmt, dtype, heads, length, starts, lens):
+    """Fresh pages, pages inside which the write begins (their scale grows or not), lengths of 0; pages and rows that no
+    token enters keep their bits; writing again changes nothing; the values read back."""
+    from lingbot_b200 import paged_cache as pc
+    b = len(starts)
+    counts = lens or [length] * b
+    need = [(s + n + 63) // 64 for s, n in zip(starts, counts)]
+    pages = P.make_pages(7 * length + heads, sum(need) + 2, heads, fmt, spread=2.5)
+    table = P.make_table(1, need, sum(need) + 2)
+    g = torch.Generator().manual_seed(length)
+    # magnitudes around the held tokens', so that some pages' scales grow and others do not
+    k, v = ((torch.randn(b, length, heads, 128, generator=g) * 2.0 ** torch.empty(b, 1, heads, 1).uniform_(-2, 1, generator=g))
+            .to(dtype) for _ in range(2))
+    got = pool(pages)
+    start = starts[0] if b == 1 else i32(starts)
+    args = (got, table.cuda(), start, k.cuda(), v.cuda())
+    pc.write(*args, lens=None if lens is None else i32(lens))
+    want = [t.clone() for t in pages]
+    P.write(want[0], want[2], table, starts, counts, k, fmt)
+    P.write(want[1], want[3], table, starts, counts, v, fmt)
+    for x, y in zip((got.k, got.v, got.k_amax, got.v_amax), want):
+        assert torch.equal(raw(x), raw(y))
+    pc.write(*args, lens=None if lens is None else i32(lens))
+    for x, y in zip((got.k, got.v, got.k_amax, got.v_amax), want):
+        assert torch.equal(raw(x), raw(y))
+    total = [s + n for s, n in zip(starts, counts)]
+    back = pc.window(got, table.cuda(), 0, max(total) or 1, dtype, lens=i32(total))
+    for x, codes, amax in zip(back, want[:2], want[2:]):
+        for s in range(b):
+            ref = P.gather(codes, amax, table[s], total[s], fmt)
+            tol = ref.abs() * (torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + 2.0 ** -23) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+            assert bool(((x[s, :total[s]].cpu().double() - ref).abs() <= tol).all())
+            assert not x[s, total[s]:].any()
+
+
+@FORMATS
+def test_write_non_finite_huge_and_tiny(fmt):
+    """NaN becomes 0 and infinities the largest code, under the scale of the finite values; magnitudes at both ends of
+    bf16; all-zero and all-NaN tokens; a subnormal below the floor."""
+    from lingbot_b200 import paged_cache as pc
+    k = torch.randn(6, 20, 2, 128, generator=torch.Generator().manual_seed(0)).bfloat16()
+    k[0, 3, 0, 5], k[0, 4, 0, 6], k[0, 5, 1, 7] = float("nan"), float("inf"), float("-inf")
+    k[1] = k[1] * 1e38
+    k[1, 0, 0, 0] = 3.3895e38
+    k[2] = k[2] * 1e-30
+    k[3] = 0
+    k[4] = float("nan")
+    k[5] = k[5] * 2.0 ** -38
+    pages = P.make_pages(3, 8, 2, fmt)
+    table = P.make_table(2, [1] * 6, 8)
+    got = pool(pages)
+    pc.write(got, table.cuda(), 0, k.cuda(), k.cuda())
+    want = [t.clone() for t in pages]
+    P.write(want[0], want[2], table, [0] * 6, [20] * 6, k, fmt)
+    for x, y in ((got.k, want[0]), (got.k_amax, want[2])):
+        assert torch.equal(raw(x), raw(y))
+    x, _ = pc.window(got, table.cuda(), 0, 20)
+    assert bool(torch.isfinite(x).all())
+
+
+@TYPES
+@pytest.mark.parametrize("interleaved,rot", [(True, 128), (False, 128), (True, 8), (False, 48)])
+def test_write_with_rope_equals_rope_then_write(dtype, interleaved, rot):
+    from lingbot_b200 import paged_cache as pc, rope
+    g = torch.Generator().manual_seed(rot)
+    qkv = torch.randn(2, 150, 3 * 3, 128, generator=g).to(dtype).cuda()
+    k, v = qkv[:, :, 3:6], qkv[:, :, 6:]                      # views of a fused projection
+    table = P.make_table(5, [4, 4], 8).cuda()
+    t = rope.tables(400, rot, interleaved=interleaved)
+    starts = i32([70, 0])
+    for positions in (None, torch.randint(0, 400, (2, 150), generator=g).cuda()):
+        a, b = (pool(P.make_pages(1, 8, 3, torch.int8)) for _ in range(2))
+        pc.write(a, table, starts, k, v, rope=t, positions=positions)
+        rows = starts[:, None] + torch.arange(150, device="cuda") if positions is None else positions
+        pc.write(b, table, starts, rope.apply(k, t, rows), v)
+        for x, y in ((a.k, b.k), (a.v, b.v), (a.k_amax, b.k_amax)):
+            assert torch.equal(raw(x), raw(y))
+
+
+def test_bad_pages_and_positions_are_recorded_not_followed():
+    from lingbot_b200 import _lib, paged_cache as pc, rope
+    pages = P.make_pages(1, 4, 2, torch.int8)
+    got = pool(pages)
+    k = torch.randn(2, 70, 2, 128).bfloat16().cuda()
+    table = torch.tensor([[0, 9], [-3, 2]], dtype=torch.int32)
+    pc.write(got, table.cuda(), 0, k, k)
+    assert _lib.device_status() == 0x305
+    want = [t.clone() for t in pages]
+    P.write(want[0], want[2], table[:1], [0], [64], k.cpu(), torch.int8)
+    P.write(want[0], want[2], torch.tensor([[0, 2]]), [64], [6], k[1:, 64:].cpu(), torch.int8)
+    assert torch.equal(raw(got.k), raw(want[0]))
+    back, _ = pc.window(got, table.cuda(), 0, 128)
+    assert _lib.device_status() == 0x305 and not back[0, 64:].any() and not back[1, :64].any() and back[1, 64:].any()
+    pc.write(got, table[:1].cuda(), i32([128]), k[:1], k[:1])                   # past the table
+    assert _lib.device_status() == 0x305
+    pc.write(got, table[:1].cuda(), i32([-5]), k[:1], k[:1])
+    assert _lib.device_status() == 0x305
+    t = rope.tables(10, 128)
+    pc.write(got, table[:1, :1].cuda().contiguous(), i32([8]), k[:1, :4], k[:1, :4], rope=t)
+    assert _lib.device_status() == 0x306
+    assert torch.equal(raw(got.v[1]), raw(pages[1][1])) and torch.equal(raw(got.v[3]), raw(pages[1][3]))
+    # attention: the keys of a bad page count as masked; lengths past the table are cut
+    q = torch.randn(2, 3, 2, 128).bfloat16().cuda()
+    out = pc.attend(q, got, table.cuda(), i32([128, 128]))
+    assert _lib.device_status() == 0x305
+    for s, (row, lo) in enumerate(((0, 0), (1, 64))):
+        good = int(table[row, 0 if s == 0 else 1])
+        one = torch.tensor([[good]], dtype=torch.int32)
+        ref, _, tol = P.attend(q[s:s + 1].cpu(), got.k.cpu(), got.v.cpu(), got.k_amax.cpu(), got.v_amax.cpu(), one, [64], [3],
+                               False)
+        assert bool(((out[s:s + 1].cpu().double() - ref).abs() <= tol + 2.0 ** -8 * ref.abs()).all())
+    pc.attend(q, got, i32([[0], [2]]), i32([65, 64]))
+    assert _lib.device_status() == 0x305
+    pc.attend(q, got, i32([[0], [2]]), i32([-1, 64]))
+    assert _lib.device_status() == 0x305
+
+
+# ------------------------------------------------------------------------------------------------ copies
+@pytest.mark.parametrize("layers,heads,total,moved", [(1, 1, 2, 1), (3, 5, 40, 17), (2, 2, 1100, 500)])
+def test_copy_pages(layers, heads, total, moved):
+    from lingbot_b200 import paged_cache as pc
+    g = torch.Generator().manual_seed(total)
+    codes = [torch.randint(-127, 128, (layers, total, heads, 64, 128), generator=g, dtype=torch.int8) for _ in range(2)]
+    amax = [torch.rand(layers, total, heads, generator=g) for _ in range(2)]
+    p = pool([*codes, *amax])
+    ids = torch.randperm(total, generator=g).tolist()
+    src, dst = ids[:moved], ids[moved:2 * moved]
+    src[-1] = src[0]                                                           # one source twice
+    pc.copy_pages(p, src, dst)
+    for x, y in zip((p.k, p.v, p.k_amax, p.v_amax), codes + amax):
+        y[:, dst] = y[:, src]
+        assert torch.equal(x.cpu(), y)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def run_attend(q, pages, table, kvs, qs, causal, **kw):
+    """Out and lse against the float64 evaluation."""
+    from lingbot_b200 import paged_cache as pc
+    p = pool(pages)
+    ragged = qs != [q.shape[1]] * q.shape[0]
+    out, lse = pc.attend(q.cuda(), p, table.cuda(), i32(kvs), q_lens=i32(qs) if ragged else None, causal=causal,
+                         return_lse=True, **kw)
+    ref, ref_lse, tol = P.attend(q, *pages, table, kvs, qs, causal, kw.get("sm_scale", 128 ** -0.5))
+    err = (out.cpu().double() - ref).abs()
+    tol = tol + torch.finfo(q.dtype).eps / 2 * ref.abs() * 1.01 + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+    assert bool((err <= tol).all()), (float((err - tol).max()), float((err / tol).max()))
+    none = ref_lse == -torch.inf
+    assert torch.equal(lse.cpu() == -torch.inf, none) and not out.cpu()[none].any()
+    # the sum of the weights is off by as much as a weight, the maximum by its score: at most 2^-11 and a rounding
+    assert bool(((lse.cpu().double() - ref_lse)[~none].abs() <= 2.0 ** -11 + 2.0 ** -20 * ref_lse[~none].abs()).all())
+    return out, lse
+
+
+@FORMATS
+@TYPES
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("kvs,lq,qs,heads,group", [
+    ([1], 1, None, 1, 1), ([64], 1, None, 2, 1), ([65, 63], 1, None, 3, 4), ([1000], 1, None, 12, 1),
+    ([300, 0, 17, 640], 5, None, 2, 3), ([300, 5, 129, 64], 9, [9, 7, 1, 0], 1, 8), ([2000], 1, None, 1, 16),
+    ([513, 900], 40, [40, 33], 2, 1), ([130], 200, None, 1, 2), ([1111], 300, None, 2, 1), ([700, 64], 257, [130, 257], 1, 3)])
+def test_attend_matches_float64(fmt, dtype, causal, kvs, lq, qs, heads, group):
+    b = len(kvs)
+    counts = [(n + 63) // 64 for n in kvs]
+    pages = P.make_pages(sum(kvs) + lq, sum(counts) + 2, heads, fmt, spread=3.0)
+    table = P.make_table(lq, counts, sum(counts) + 2, width=max(counts) + 3)
+    g = torch.Generator().manual_seed(lq)
+    q = (torch.randn(b, lq, heads * group, 128, generator=g) * 1.5).to(dtype)
+    run_attend(q, pages, table, kvs, qs or [lq] * b, causal)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 16, 40])
+@pytest.mark.parametrize("lq,group", [(1, 1), (4, 8), (150, 2)])
+def test_attend_key_splits(splits, lq, group):
+    """Every split count, uneven ones and more than there are pages among them; sequences that end in the first split."""
+    kvs = [1000, 40, 0, 641]
+    pages = P.make_pages(11, 40, 2, torch.int8, spread=2.0)
+    table = P.make_table(4, [16, 1, 0, 11], 40)
+    q = torch.randn(4, lq, 2 * group, 128, generator=torch.Generator().manual_seed(1)).bfloat16()
+    run_attend(q, pages, table, kvs, [lq] * 4, True, num_splits=splits)
+
+
+@FORMATS
+@pytest.mark.parametrize("lq", [1, 129], ids=["token", "chunk"])
+def test_attend_wide_ranges(fmt, lq):
+    """Pages whose V differ by 2^12 and K by 2^4, large query rows beside tiny ones, a softmax that picks one key."""
+    kvs = [600]
+    k, v, ka, va = P.make_pages(5, 10, 1, fmt, spread=4.0)
+    va = 2.0 ** (torch.arange(10.0) * 12 / 9 - 6)[:, None]
+    table = P.make_table(9, [10], 10)
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(1, lq, 2, 128, generator=g)
+    q[:, :, 1] *= 30
+    q[:, ::2, 0] *= 2.0 ** -60
+    run_attend(q.bfloat16(), (k, v, ka, va), table, kvs, [lq], False)
+    run_attend(q.bfloat16(), (k, v, ka, va), table, kvs, [lq], False, sm_scale=1.5)
+
+
+@pytest.mark.parametrize("lq", [1, 130], ids=["token", "chunk"])
+def test_attend_strides_stale_rows_and_padding(lq):
+    """q and out as views of larger tensors; garbage past a sequence's tokens, in other pages and in padded query rows
+    (NaN there) changes nothing; rows past q_lens are 0; a broadcast query; a shared page table row."""
+    from lingbot_b200 import paged_cache as pc
+    kvs, qs = [100, 190], [max(1, lq - 3), lq]
+    pages = P.make_pages(8, 8, 2, torch.float8_e4m3fn)
+    table = P.make_table(3, [2, 3], 8)
+    g = torch.Generator().manual_seed(0)
+    big = torch.randn(2, lq, 3, 4, 128, generator=g).bfloat16().cuda()
+    q = big[:, :, 1]
+    p = pool(pages)
+    want = pc.attend(q.contiguous(), p, table.cuda(), i32(kvs), q_lens=i32(qs))
+    assert not want[0, qs[0]:].any()
+    hold = torch.full((2, lq, 6, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = pc.attend(q, p, table.cuda(), i32(kvs), q_lens=i32(qs), out=hold[:, :, 1:5])
+    assert torch.equal(got, want) and bool((hold[:, :, 0] == 7).all()) and bool((hold[:, :, 5] == 7).all())
+    k2, v2 = (t.clone() for t in pages[:2])
+    for t in (k2, v2):
+        raw_t = t.view(torch.uint8)
+        raw_t[table[0, 1].item(), :, 36:] = 0x7F                              # NaN codes behind the last token
+        raw_t[[i for i in range(8) if i not in table.flatten().tolist()]] = 0xFF
+    q2 = q.clone()
+    q2[0, qs[0]:] = float("nan")
+    again = pc.attend(q2, pool((k2, v2, *pages[2:])), table.cuda(), i32(kvs), q_lens=i32(qs))
+    assert torch.equal(again, want)
+    wide = torch.full((2, 50), -1, dtype=torch.int32)
+    wide[:, :3] = table
+    same = pc.attend(q, p, wide.cuda(), i32(kvs), q_lens=i32(qs), max_kv_len=190)
+    assert torch.equal(same, want)
+    e = q[:1].expand(2, lq, 4, 128)
+    shared = table[1:].cuda().expand(2, 3)
+    both = pc.attend(e, p, shared, 190)
+    assert torch.equal(both[0], both[1])
+
+
+def test_attend_rows_with_nan_or_inf_stay_alone():
+    from lingbot_b200 import paged_cache as pc
+    for lq in (4, 140):
+        pages = P.make_pages(8, 4, 1, torch.int8)
+        table = P.make_table(3, [4], 4).cuda()
+        q = torch.randn(1, lq, 2, 128, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+        want = pc.attend(q, pool(pages), table, 250)
+        q[0, 1, 0, 3] = float("nan")
+        q[0, 2, 1, 9] = float("inf")
+        got = pc.attend(q, pool(pages), table, 250)
+        assert bool(got[0, 1, 0].isnan().all()) and bool(got[0, 2, 1].isnan().any())
+        keep = torch.ones(lq, 2, dtype=torch.bool, device="cuda")
+        keep[1, 0] = keep[2, 1] = False
+        assert torch.equal(got[0][keep], want[0][keep])
+
+
+def test_pool_larger_than_32_bits_of_bytes():
+    """Pages behind the first 4 GiB of each tensor: written, read, copied and attended."""
+    from lingbot_b200 import paged_cache as pc
+    n, h = 45000, 12                                                           # 4.4 GB a tensor
+    p = pc.alloc_pages(n, h, "cuda")
+    ids = [n - 1, 3, n - 7, 20000]
+    table = i32([ids])
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(1, 250, h, 128, generator=g).bfloat16().cuda() for _ in range(2))
+    pc.write(p, table, 0, k, v)
+    small = pc.alloc_pages(4, h, "cuda")
+    pc.write(small, i32([[0, 1, 2, 3]]), 0, k, v)
+    for a, b in ((p.k, small.k), (p.v, small.v), (p.k_amax, small.k_amax)):
+        assert torch.equal(a[ids], b)
+    for lq in (1, 150):
+        q = torch.randn(1, lq, h, 128, generator=g).bfloat16().cuda()
+        assert torch.equal(pc.attend(q, p, table, 250), pc.attend(q, small, i32([[0, 1, 2, 3]]), 250))
+    pc.copy_pages(p, [n - 1, n - 7], [5, n - 2])
+    assert torch.equal(p.k[5], small.k[0]) and torch.equal(p.v[n - 2], small.v[2])
+    x, y = pc.window(p, table, 0, 250), pc.window(small, i32([[0, 1, 2, 3]]), 0, 250)
+    assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+
+
+def test_streams_graphs_and_gradients():
+    """Calls on two streams at once, and two captured graphs replayed in turn on changing lengths, give what eager calls
+    give; a query that needs a gradient is refused."""
+    from lingbot_b200 import paged_cache as pc
+    pages = P.make_pages(8, 40, 4, torch.int8)
+    p = pool(pages)
+    table = P.make_table(3, [16, 16], 40).cuda()
+    g = torch.Generator().manual_seed(0)
+    qs = [torch.randn(2, lq, 8, 128, generator=g).bfloat16().cuda() for lq in (1, 3, 140)]
+    lens = i32([1000, 700])
+    want = [pc.attend(q, p, table, lens, causal=True) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for r in range(6):
+        with torch.cuda.stream(streams[r % 2]):
+            got += [pc.attend(q, p, table, lens, causal=True) for q in qs]
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, want[i % 3])
+    graphs, outs = [], []
+    for q in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(pc.attend(q, p, table, lens, causal=True))
+        graphs.append(graph)
+    for new in ([1000, 700], [3, 0], [64, 1024]):
+        lens.copy_(i32(new))
+        for r in range(2):
+            for graph in graphs:
+                graph.replay()
+        torch.cuda.synchronize()
+        for q, x in zip(qs, outs):
+            assert torch.equal(x, pc.attend(q, p, table, i32(new), causal=True))
+    with pytest.raises(RuntimeError, match="gradient"):
+        pc.attend(qs[0].clone().requires_grad_(), p, table, lens)
+
+
+# ------------------------------------------------------------------------------------------------ the cache as used
+@FORMATS
+def test_sessions_prefill_decode_fork_evict_compact(fmt):
+    """Two layers: a prompt, generated tokens with rope, a fork that goes its own way, an eviction, compaction, a captured
+    decode step; every attention against float64 on a model that keeps the sessions' codes as the formulas give them."""
+    from lingbot_b200 import paged_cache as pc, rope
+    heads, group, layers = 2, 2, 2
+    c = pc.allocate(layers, 24, heads, max_pages=8, device="cuda", fmt=fmt)
+    t = rope.tables(600, 64, interleaved=False)
+    g = torch.Generator().manual_seed(5)
+
+    def rand(b, n, h):
+        return torch.randn(b, n, h, 128, generator=g).bfloat16().cuda()
+
+    def step(sessions, new, causal=True, passes=1):
+        plan = c.plan(sessions, new)
+        b, n = len(sessions), max(plan.new)
+        for layer in range(layers):
+            for _ in range(passes):
+                k, v, q = rand(b, n, heads), rand(b, n, heads), rand(b, n, heads * group)
+                before = [x.cpu() for x in (c.layers[layer].k, c.layers[layer].v, c.layers[layer].k_amax, c.layers[layer].v_amax)]
+                rows = plan.start[:, None] + torch.arange(n, device="cuda")
+                c.write(layer, plan, k, v, rope=t)
+                kr = rope.apply(k, t, rows)
+                table = plan.table.cpu()
+                P.write(before[0], before[2], table, plan.held, plan.new, kr.cpu(), fmt)
+                P.write(before[1], before[3], table, plan.held, plan.new, v.cpu(), fmt)
+                qr = rope.apply(q, t, rows)
+                out = c.attend(layer, plan, qr, causal=causal)
+                kvs = [h + m for h, m in zip(plan.held, plan.new)]
+                ref, _, tol = P.attend(qr.cpu(), *before, table, kvs, plan.new, causal)
+                assert bool(((out.cpu().double() - ref).abs() <= tol + 2.0 ** -8 * ref.abs() * 1.01).all())
+                for x, y in zip((c.layers[layer].k, c.layers[layer].v), before):
+                    assert torch.equal(raw(x), raw(y))
+        c.commit(plan)
+        return plan
+
+    a, b = c.open(), c.open()
+    step([a, b], [200, 131])
+    step([a, b], 1)
+    f = c.fork(a)
+    step([a, f, b], [3, 1, 64], causal=False, passes=2)
+    assert c.page_ids(a)[:3] == c.page_ids(f)[:3] and c.page_ids(a)[3] != c.page_ids(f)[3]
+    kept = [c.layers[i].k[c.page_ids(a)].cpu() for i in range(layers)]
+    c.evict(f, 64, 64)
+    c.close(b)
+    assert c.compact() > 0
+    assert max(c.page_ids(a) + c.page_ids(f)) == c.num_pages - c.free_pages - 1
+    for i in range(layers):
+        assert torch.equal(raw(c.layers[i].k[c.page_ids(a)]), raw(kept[i]))
+    step([f, a], [1, 5])
+    # a captured decode step: the plan's tensors take the next step's values
+    plan = c.fixed_plan(2)
+    k, v, q = rand(2, 1, heads), rand(2, 1, heads), rand(2, 1, heads * group)
+    c.plan([a, f], 1, into=plan)
+    c.write(0, plan, k, v, rope=t)
+    c.attend(0, plan, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.write(0, plan, k, v, rope=t)
+        out = c.attend(0, plan, q, causal=True)
+    for _ in range(3):
+        for x, h in ((k, heads), (v, heads), (q, heads * group)):
+            x.copy_(rand(2, 1, h))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = pc.attend(q, c.layers[0], plan.table, plan.kv_lens, causal=True, num_splits=1)
+        assert torch.allclose(out.float(), eager.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+        c.commit(plan)
+        c.plan([a, f], 1, into=plan)
