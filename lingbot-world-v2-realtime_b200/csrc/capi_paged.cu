@@ -74,11 +74,10 @@ int finish(cudaError_t e, const char* what) {
   return e == cudaSuccess ? LBQ_OK : set_error(LBQ_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-// Query rows (token, query head of the K/V head) that one CTA of the attention kernel takes.
-int attn_tile_rows(int64_t rows) {
-  (void)rows;
-  return 16;
-}
+// Query rows (token, query head of the K/V head) that one CTA takes, by the rows of a K/V head: the few-row kernel up
+// to kFewRows, the many-row kernel above.
+constexpr int64_t kFewRows = 64;
+int attn_tile_rows(int64_t rows) { return rows <= kFewRows ? lbq::kFewTile : lbq::kManyTile; }
 
 }  // namespace
 
@@ -263,9 +262,11 @@ int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t ma
   const int tile = attn_tile_rows(rows);
   const int64_t ctas = (rows + tile - 1) / tile * heads * batch;
   const int64_t pages = (max_kv_len + lbq::kPageTokens - 1) / lbq::kPageTokens;
-  // two CTAs an SM; a split keeps at least 4 pages, one for each warp
-  int64_t n = 2 * 148 / ctas;
-  if (n > pages / 4) n = pages / 4;
+  // few rows: two CTAs an SM, a split keeps at least 4 pages, one for each warp; many rows: one CTA an SM, at least
+  // 8 pages (4 key tiles) to pay for the query tiles
+  int64_t n = (tile == lbq::kFewTile ? 2 * 148 : 148) / ctas;
+  const int64_t least = tile == lbq::kFewTile ? 4 : 8;
+  if (n > pages / least) n = pages / least;
   return int(n < 1 ? 1 : (n > 1024 ? 1024 : n));
 }
 
@@ -319,11 +320,6 @@ int lbq_paged_attn(const void* q, int64_t sq_b, int64_t sq_l, int64_t sq_h, cons
     a.o_part = static_cast<float*>(workspace);
     a.ml_part = reinterpret_cast<float2*>(a.o_part + n * 128);
   }
-  CUtensorMap tk, tv;
-  const uint64_t prows = uint64_t(num_pages) * heads * lbq::kPageTokens;
-  if ((r = lbq::make_page_map(&tk, k_pages, prows, "k_pages", lbq::kPageTokens)) ||
-      (r = lbq::make_page_map(&tv, v_pages, prows, "v_pages", lbq::kPageTokens)))
-    return r;
   if (!(sm_scale > 0.f)) sm_scale = 0.08838834764831845f;   // 128 ** -0.5
   a.q = q;
   a.out = out;
@@ -336,6 +332,9 @@ int lbq_paged_attn(const void* q, int64_t sq_b, int64_t sq_l, int64_t sq_h, cons
   a.ka = k_amax;
   a.va = v_amax;
   a.pt = lbq::PageTable{table, st_b, width, num_pages};
+  a.k_pages = static_cast<const uint8_t*>(k_pages);
+  a.v_pages = static_cast<const uint8_t*>(v_pages);
+  a.wide_out = aligned(out, 32) && so_b % 16 == 0 && so_l % 16 == 0 && so_h % 16 == 0;
   a.kv_lens = kv_lens;
   a.kv_len0 = kv_len0;
   a.q_lens = q_lens;
@@ -350,7 +349,17 @@ int lbq_paged_attn(const void* q, int64_t sq_b, int64_t sq_l, int64_t sq_h, cons
   a.v_unit = 1.f / lbq::code_max(fmt);
   a.status = lbq::device_status_ptr();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if ((r = finish(lbq::launch_paged_decode(a, tk, tv, st), "paged_attn launch"))) return r;
+  if (a.tile_rows == lbq::kFewTile) {
+    CUtensorMap tk, tv;
+    const uint64_t prows = uint64_t(num_pages) * heads * lbq::kPageTokens;
+    if ((r = lbq::make_page_map(&tk, k_pages, prows, "k_pages", lbq::kPageTokens)) ||
+        (r = lbq::make_page_map(&tv, v_pages, prows, "v_pages", lbq::kPageTokens)))
+      return r;
+    r = finish(lbq::launch_paged_decode(a, tk, tv, st), "paged_attn launch");
+  } else {
+    r = finish(lbq::launch_paged_rows(a, st), "paged_attn launch");
+  }
+  if (r) return r;
   if (a.splits > 1) return finish(lbq::launch_paged_combine(a, st), "paged_attn merge launch");
   return LBQ_OK;
 }

@@ -1,0 +1,55 @@
+// Device pieces that the two attention kernels over the paged cache share.
+#pragma once
+#include <cuda_fp16.h>
+#include <cstdint>
+
+#include "lbq_paged.h"
+#include "lbq_ptx.cuh"
+
+namespace lbq {
+
+// Keys [0, visible) are seen by some row of the tile; 0 when every row is empty or past the sequence's queries.
+struct TileKeys {
+  int64_t kv;
+  int qn;
+  int64_t visible;
+};
+__device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, int b, int tile) {
+  TileKeys t;
+  t.kv = a.kv_lens ? a.kv_lens[b] : a.kv_len0;
+  const int64_t most = int64_t(a.pt.width) * kPageTokens;
+  if (t.kv < 0 || t.kv > most) {
+    if (a.status) atomicCAS(a.status, 0, kDevBadPage);
+    t.kv = t.kv < 0 ? 0 : most;
+  }
+  t.qn = a.q_lens ? a.q_lens[b] : a.q_len;
+  t.qn = t.qn < 0 ? 0 : (t.qn > a.q_len ? a.q_len : t.qn);
+  const int first = tile * a.tile_rows / a.group;                        // first and last query token of the tile
+  const int last = min((tile * a.tile_rows + a.tile_rows - 1) / a.group, t.qn - 1);
+  if (first > last) t.visible = 0;
+  else t.visible = a.causal ? min(t.kv, max(t.kv - t.qn + last + 1, int64_t(0))) : t.kv;
+  return t;
+}
+
+// Bytes (s0, s1) of r as a pair of fp16 values: int8 through 1024 + (c + 128), exact; e4m3 by the converter.
+template <int kFmt, int kS0, int kS1>
+__device__ __forceinline__ uint32_t widen(uint32_t r) {
+  uint32_t d;
+  if constexpr (kFmt == 0) {
+    const uint32_t p = __byte_perm(r, 0x64646464u, 0x4040 | kS0 | (kS1 << 8));
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&p), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+    d = *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const uint16_t p = uint16_t(__byte_perm(r, 0u, kS0 | (kS1 << 4)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(p));
+  }
+  return d;
+}
+template <int kFmt>
+__device__ __forceinline__ uint32_t bias(uint32_t r) { return kFmt == 0 ? r ^ 0x80808080u : r; }
+
+__device__ __forceinline__ float natural_lse(float m, float l) {
+  return l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : (l == l ? -INFINITY : l);
+}
+
+}  // namespace lbq

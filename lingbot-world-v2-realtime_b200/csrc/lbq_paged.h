@@ -77,6 +77,8 @@ struct PageReadArgs {
   int* status;
 };
 
+constexpr int kFewTile = 16, kManyTile = 256;   // query rows of a CTA: few-row and many-row attention kernels
+
 constexpr int kCopyPairs = 480;               // page pairs of one launch (they travel as kernel parameters)
 struct PageCopyArgs {
   uint8_t* codes[2];
@@ -92,6 +94,8 @@ struct PagedAttnArgs {
   void* out;
   int64_t so[3];
   float* lse;                   // null, or [B, Lq, heads * group]
+  const uint8_t* k_pages;
+  const uint8_t* v_pages;
   const float* ka;
   const float* va;
   PageTable pt;
@@ -105,6 +109,7 @@ struct PagedAttnArgs {
   int splits, split_pages;      // key splits, and the pages of one
   float* o_part;                // [splits][batch * heads][tiles * tile_rows][128] (splits > 1)
   float2* ml_part;              // the same rows' (max in log2 units, sum)
+  int wide_out;                 // out's base and strides are 32-byte aligned
   int* status;
 };
 
@@ -114,6 +119,7 @@ cudaError_t launch_page_read(const PageReadArgs& a, cudaStream_t st);
 cudaError_t launch_page_copy(const PageCopyArgs& a, cudaStream_t st);
 cudaError_t launch_paged_decode(const PagedAttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                                 cudaStream_t st);
+cudaError_t launch_paged_rows(const PagedAttnArgs& a, cudaStream_t st);
 cudaError_t launch_paged_combine(const PagedAttnArgs& a, cudaStream_t st);
 
 // Tensor map of `rows` x 128 bytes, box 64 x 128 bytes, 128-byte swizzle; 0 or an LBQ_ERR_* code.

@@ -220,6 +220,24 @@ __device__ __forceinline__ void mma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// D[tmem] (+)= A[smem] * B[smem], f16 x f16 -> fp32.
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A in tensor memory: lane = row, a 32-bit column holds two consecutive K elements.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // Makes this thread's generic-proxy shared-memory writes visible to the async proxy (TMA, tcgen05).
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -239,6 +257,12 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// MN-major operand, 128-byte swizzle: rows of 128 bytes run along MN, 8 K rows to a 1024-byte group, the next 128 bytes
+// of MN `mn_stride` bytes on.
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t smem_addr, uint32_t mn_stride) {
+  return (smem_desc_sw128(smem_addr) & ~(uint64_t(0x3FFF) << 16)) | (uint64_t((mn_stride >> 4) & 0x3FFF) << 16);
+}
+
 // Instruction descriptors (M=128, both operands K-major, dense).
 //   [4,6) D format (1 = f32, 2 = s32), [7,10) A format, [10,13) B format,
 //   [17,23) N>>3, [24,29) M>>4.
@@ -246,6 +270,8 @@ constexpr uint32_t idesc_m128(uint32_t n, uint32_t dfmt, uint32_t afmt, uint32_t
   return (dfmt << 4) | (afmt << 7) | (bfmt << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 constexpr uint32_t kIdescQK = idesc_m128(128, 2, 1, 1);   // s32 <- s8 x s8, N = 128 keys
+constexpr uint32_t kIdescF16 = idesc_m128(128, 1, 0, 0);                  // f32 <- f16 x f16, both K-major
+constexpr uint32_t kIdescF16BMn = kIdescF16 | (1u << 16);                // B MN-major
 constexpr uint32_t kIdescPV = idesc_m128(128, 1, 0, 0);   // f32 <- e4m3 x e4m3, N = 128 channels
 
 // Warp-collective TMEM load: thread i of the warp reads lane (lane_base + i), 32 consecutive

@@ -21,6 +21,7 @@
 
 #include "lbq_kernels.h"
 #include "lbq_paged.h"
+#include "lbq_paged.cuh"
 #include "lbq_ptx.cuh"
 
 namespace lbq {
@@ -31,29 +32,6 @@ constexpr int kDecRows = 16;
 constexpr int kMergePitch = 132;                       // floats of a merged row in shared memory
 constexpr size_t kDecSmem = 1024 + size_t(kDecSlots) * 2 * kPageBytes;
 static_assert(size_t(kDecWarps) * kDecRows * kMergePitch * 4 <= size_t(kDecSlots) * 2 * kPageBytes, "merge area");
-
-// Keys [0, visible) are seen by some row of the tile; 0 when every row is empty or past the sequence's queries.
-struct TileKeys {
-  int64_t kv;
-  int qn;
-  int64_t visible;
-};
-__device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, int b, int tile) {
-  TileKeys t;
-  t.kv = a.kv_lens ? a.kv_lens[b] : a.kv_len0;
-  const int64_t most = int64_t(a.pt.width) * kPageTokens;
-  if (t.kv < 0 || t.kv > most) {
-    if (a.status) atomicCAS(a.status, 0, kDevBadPage);
-    t.kv = t.kv < 0 ? 0 : most;
-  }
-  t.qn = a.q_lens ? a.q_lens[b] : a.q_len;
-  t.qn = t.qn < 0 ? 0 : (t.qn > a.q_len ? a.q_len : t.qn);
-  const int first = tile * a.tile_rows / a.group;                        // first and last query token of the tile
-  const int last = min((tile * a.tile_rows + a.tile_rows - 1) / a.group, t.qn - 1);
-  if (first > last) t.visible = 0;
-  else t.visible = a.causal ? min(t.kv, max(t.kv - t.qn + last + 1, int64_t(0))) : t.kv;
-  return t;
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -72,23 +50,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Bytes (s0, s1) of r as a pair of fp16 values: int8 through 1024 + (c + 128), exact; e4m3 by the converter.
-template <int kFmt, int kS0, int kS1>
-__device__ __forceinline__ uint32_t widen(uint32_t r) {
-  uint32_t d;
-  if constexpr (kFmt == 0) {
-    const uint32_t p = __byte_perm(r, 0x64646464u, 0x4040 | kS0 | (kS1 << 8));
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&p), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-    d = *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const uint16_t p = uint16_t(__byte_perm(r, 0u, kS0 | (kS1 << 4)));
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(p));
-  }
-  return d;
-}
-template <int kFmt>
-__device__ __forceinline__ uint32_t bias(uint32_t r) { return kFmt == 0 ? r ^ 0x80808080u : r; }
-
 // Channels 4 * (lane % 4) .. + 3 of every 16 of one query row as the A fragments of 8 MMA steps (the channel order
 // inside a step is the one in which ldmatrix hands out four consecutive bytes of K; a dot product does not mind),
 // scaled by a power of two to a largest magnitude in [1, 2); returns the factor that undoes it.
@@ -138,10 +99,6 @@ __device__ __forceinline__ void store_out16(const PagedAttnArgs& a, int b, int i
   reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
   reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
-__device__ __forceinline__ float natural_lse(float m, float l) {
-  return l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : (l == l ? -INFINITY : l);
-}
-
 struct DecShared {
   uint64_t full[kDecSlots];
   int issued[kDecSlots];

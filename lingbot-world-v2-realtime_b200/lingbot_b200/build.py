@@ -12,8 +12,8 @@ CSRC = os.path.join(ROOT, "csrc")
 LIB = os.path.join(PKG_DIR, "liblbq.so")
 DEBUG_LIB = os.path.join(PKG_DIR, "liblbq_debug.so")
 SOURCES = ["quant.cu", "attn.cu", "fp8lin.cu", "capi.cu", "noalloc.cu", "peer.cu", "capi_peer.cu",
-           "rope.cu", "paged.cu", "pattn.cu", "capi_paged.cu"]
-HEADERS = ["lbq_ptx.cuh", "lbq_kernels.h", "lbq_peer.cuh", "lbq_paged.h", os.path.join("..", "..", "include", "lbq.h")]
+           "rope.cu", "paged.cu", "pattn.cu", "prows.cu", "capi_paged.cu"]
+HEADERS = ["lbq_ptx.cuh", "lbq_kernels.h", "lbq_peer.cuh", "lbq_paged.h", "lbq_paged.cuh", os.path.join("..", "..", "include", "lbq.h")]
 
 
 def nvcc():

@@ -51,8 +51,13 @@ class Pages:
                              f"got {tuple(k.shape)}, {tuple(v.shape)}, {tuple(ka.shape)}, {tuple(va.shape)}")
         if not (k.is_contiguous() and v.is_contiguous() and ka.is_contiguous() and va.is_contiguous()):
             raise ValueError("pages must be contiguous")
-        if not k.is_cuda or any(t.device != k.device for t in (v, ka, va)):
+        dev = k.device
+        if not k.is_cuda or v.device != dev or ka.device != dev or va.device != dev:
             raise ValueError("pages must be CUDA tensors of one device")
+        self.device = dev
+        self.heads = k.shape[-3]
+        self._args = None if k.dim() == 5 else (k.data_ptr(), ka.data_ptr(), v.data_ptr(), va.data_ptr(), k.shape[0],
+                                                self.heads, FORMATS[k.dtype])
 
     def layer(self, i) -> "Pages":
         """The pool of one layer."""
@@ -60,11 +65,11 @@ class Pages:
             raise ValueError("the pool has no layers")
         return Pages(self.k[i], self.v[i], self.k_amax[i], self.v_amax[i])
 
-    def _args(self):
-        if self.k.dim() != 4:
+    def args(self):
+        """The pool's arguments of the C ABI."""
+        if self._args is None:
             raise ValueError("the pool has layers: take .layer(i)")
-        return (self.k.data_ptr(), self.k_amax.data_ptr(), self.v.data_ptr(), self.v_amax.data_ptr(), self.k.shape[0],
-                self.k.shape[1], FORMATS[self.k.dtype])
+        return self._args
 
 
 def alloc_pages(num_pages, heads, device, fmt=torch.int8, layers=None) -> Pages:
@@ -77,18 +82,22 @@ def alloc_pages(num_pages, heads, device, fmt=torch.int8, layers=None) -> Pages:
     return Pages(*codes, *amax)
 
 
-def _table(page_table, batch, device):
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch \
-            or page_table.stride(1) != 1 or page_table.device != device or page_table.shape[1] == 0:
-        raise ValueError(f"page table: an int32 [{batch}, pages] tensor on {device} with unit last stride, got "
-                         f"{page_table.dtype} {tuple(page_table.shape)} on {page_table.device}")
-    return page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
+def _table(t, batch, device):
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.device != device:
+        raise ValueError(f"page table: an int32 [batch, pages] tensor on {device}, got {t.dtype} {tuple(t.shape)} on "
+                         f"{t.device}")
+    n, width = t.shape
+    row, unit = t.stride()
+    if n != batch or width == 0 or (unit != 1 and width > 1):
+        raise ValueError(f"page table: [{batch}, pages] with unit last stride, got {tuple(t.shape)}, strides {t.stride()}")
+    return t.data_ptr(), row, width
 
 
 def _counts(name, t, batch, device):
     """A count for each sequence: (pointer, 0) of an int32 [batch] tensor, (None, value) of an int."""
     if isinstance(t, torch.Tensor):
-        if t.dtype != torch.int32 or tuple(t.shape) != (batch,) or t.device != device or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != batch or t.device != device \
+                or (batch > 1 and t.stride(0) != 1):
             raise ValueError(f"{name}: a contiguous int32 [{batch}] tensor on {device}, got {t.dtype} {tuple(t.shape)} on "
                              f"{t.device}")
         return t.data_ptr(), 0
@@ -98,19 +107,17 @@ def _counts(name, t, batch, device):
     return None, t
 
 
-def _check_rows(name, x, pages, heads=None):
+def _check_rows(name, x, device):
     if x.dtype not in _ACT:
         raise TypeError(f"{name} must be bfloat16 or float16, got {x.dtype}")
     if x.dim() != 4 or x.shape[3] != HEAD_DIM or x.stride(3) != 1:
         raise ValueError(f"{name} must be [B, L, heads, {HEAD_DIM}] with unit channel stride, got {tuple(x.shape)}")
-    if x.device != pages.k.device:
-        raise ValueError(f"{name} on {x.device}, pages on {pages.k.device}")
-    if heads is not None and x.shape[2] != heads:
-        raise ValueError(f"{name} has {x.shape[2]} heads, the pages {heads}")
+    if x.device != device:
+        raise ValueError(f"{name} on {x.device}, pages on {device}")
 
 
-def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _no_grad():
+    if torch.is_grad_enabled():
         raise RuntimeError("the paged cache records no gradient: call it under torch.no_grad()")
 
 
@@ -120,17 +127,17 @@ def write(pages: Pages, page_table, start, k, v, lens=None, rope: Rope = None, p
     keeps them: when its largest magnitude grows their codes are rounded to the new scale. Tokens at and past `start`
     are replaced. With `rope`, K is rotated on the way, by `positions` [B, L] or its token indices, to the same bits as
     rope.apply followed by a plain write. Two sequences of one call must not write the same page."""
-    args = pages._args()
-    heads = args[5]
-    _check_rows("k", k, pages, heads)
-    _check_rows("v", v, pages, heads)
-    if v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ")
-    _no_grad(k, v)
+    args, heads, dev = pages.args(), pages.heads, pages.device
+    _check_rows("k", k, dev)
+    _check_rows("v", v, dev)
+    if v.shape != k.shape or v.dtype != k.dtype or k.shape[2] != heads:
+        raise ValueError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ, or are not of the pages' "
+                         f"{heads} heads")
+    if k.requires_grad or v.requires_grad:
+        _no_grad()
     b, l = k.shape[:2]
     if b == 0 or l == 0:
         return
-    dev = k.device
     table = _table(page_table, b, dev)
     sp, s0 = _counts("start", start, b, dev)
     lp = None
@@ -149,29 +156,33 @@ def write(pages: Pages, page_table, start, k, v, lens=None, rope: Rope = None, p
     else:
         if positions is not None and positions.shape[-1] > l:
             positions = positions[..., :l]
-        turn = rope.args(positions, dev, (b, l))
-    _lib.call_on(dev, "lbq_page_write", k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], *args, *table, sp, s0,
-                 lp, b, l, *turn, _ACT[k.dtype])
+        turn = rope.args(positions, dev, b, l)
+    sk, sv = k.stride(), v.stride()
+    _lib.call_on(dev, "lbq_page_write", k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2], *args, *table,
+                 sp, s0, lp, b, l, *turn, _ACT[k.dtype])
 
 
 def window(pages: Pages, page_table, start, length, dtype=torch.bfloat16, lens=None, out=None):
     """Values (k, v) [B, length, heads, 128] in `dtype` of the tokens from start[b] on; rows past lens[b] (None: all) are
     0. The role of kv_cache.window, as a copy."""
-    args = pages._args()
-    heads, dev = args[5], pages.k.device
+    args, heads, dev = pages.args(), pages.heads, pages.device
     b, length = page_table.shape[0], int(length)
     if dtype not in _ACT:
         raise TypeError(f"window dtype {dtype}: expected bfloat16 or float16")
     if length < 0:
         raise ValueError(f"length {length} is negative")
     if out is None:
-        out = tuple(torch.empty(b, length, heads, HEAD_DIM, dtype=dtype, device=dev) for _ in range(2))
-    for name, t in zip(("k out", "v out"), out):
-        _check_rows(name, t, pages, heads)
-        if tuple(t.shape[:2]) != (b, length) or t.dtype != dtype:
-            raise ValueError(f"{name} must be {dtype} [{b}, {length}, {heads}, {HEAD_DIM}], got {t.dtype} {tuple(t.shape)}")
+        k = torch.empty((b, length, heads, HEAD_DIM), dtype=dtype, device=dev)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
+        for name, t in (("k out", k), ("v out", v)):
+            _check_rows(name, t, dev)
+            if tuple(t.shape[:3]) != (b, length, heads) or t.dtype != dtype:
+                raise ValueError(f"{name} must be {dtype} [{b}, {length}, {heads}, {HEAD_DIM}], got {t.dtype} "
+                                 f"{tuple(t.shape)}")
     if b == 0 or length == 0:
-        return out
+        return k, v
     table = _table(page_table, b, dev)
     sp, s0 = _counts("start", start, b, dev)
     lp = None
@@ -179,10 +190,10 @@ def window(pages: Pages, page_table, start, length, dtype=torch.bfloat16, lens=N
         if not isinstance(lens, torch.Tensor):
             lens = torch.full((b,), int(lens), dtype=torch.int32, device=dev)
         lp, _ = _counts("lens", lens, b, dev)
-    k, v = out
-    _lib.call_on(dev, "lbq_page_read", *args, *table, sp, s0, lp, b, length, k.data_ptr(), *k.stride()[:3], v.data_ptr(),
-                 *v.stride()[:3], _ACT[dtype])
-    return out
+    sk, sv = k.stride(), v.stride()
+    _lib.call_on(dev, "lbq_page_read", *args, *table, sp, s0, lp, b, length, k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(),
+                 sv[0], sv[1], sv[2], _ACT[dtype])
+    return k, v
 
 
 def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_scale=None, out=None, return_lse=False,
@@ -193,20 +204,21 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
     a padded batch. Rows that see no token, and rows past q_lens[b], are 0. Returns out [B, Lq, heads, 128] in q's dtype,
     with return_lse also the rows' log-sum-exp f32 [B, Lq, heads] (-inf for those rows). max_kv_len bounds kv_lens where
     the page table is much wider than the longest sequence; num_splits overrides the number of key splits."""
-    args = pages._args()
-    _check_rows("q", q, pages)
-    b, lq, hq = q.shape[:3]
-    heads, dev = args[5], q.device
-    if hq % heads or hq == 0:
+    args, heads, dev = pages.args(), pages.heads, pages.device
+    _check_rows("q", q, dev)
+    b, lq, hq, _ = q.shape
+    group = hq // heads
+    if group * heads != hq or hq == 0:
         raise ValueError(f"q has {hq} heads, not a multiple of the pages' {heads}")
-    _no_grad(q)
+    if q.requires_grad:
+        _no_grad()
     if out is None:
-        out = torch.empty(b, lq, hq, HEAD_DIM, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q)
     else:
-        _check_rows("out", out, pages, hq)
+        _check_rows("out", out, dev)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
-    lse = torch.empty(b, lq, hq, dtype=torch.float32, device=dev) if return_lse else None
+    lse = torch.empty((b, lq, hq), dtype=torch.float32, device=dev) if return_lse else None
     if b and lq:
         tp, ts, width = _table(page_table, b, dev)
         kp, k0 = _counts("kv_lens", kv_lens, b, dev)
@@ -222,7 +234,6 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
                 width = max(1, min(width, (longest + PAGE - 1) // PAGE))
             elif k0 > longest:
                 raise ValueError(f"kv_lens {k0} exceeds max_kv_len {longest}")
-        group = hq // heads
         lib = _lib.load()
         if num_splits is None:
             num_splits = lib.lbq_paged_attn_splits(b, lq, heads, group, longest)
@@ -230,8 +241,9 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
         if num_splits > 1:
             ws_bytes = lib.lbq_paged_attn_workspace(b, lq, heads, group, num_splits)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        _lib.call_on(dev, "lbq_paged_attn", q.data_ptr(), *q.stride()[:3], *args, tp, ts, width, kp, k0, qp, b, lq, group,
-                     int(bool(causal)), float(sm_scale or 0.0), out.data_ptr(), *out.stride()[:3],
+        sq, so = q.stride(), out.stride()
+        _lib.call_on(dev, "lbq_paged_attn", q.data_ptr(), sq[0], sq[1], sq[2], *args, tp, ts, width, kp, k0, qp, b, lq, group,
+                     1 if causal else 0, float(sm_scale or 0.0), out.data_ptr(), so[0], so[1], so[2],
                      None if lse is None else lse.data_ptr(), num_splits, None if ws is None else ws.data_ptr(), ws_bytes,
                      _ACT[q.dtype])
     return (out, lse) if return_lse else out

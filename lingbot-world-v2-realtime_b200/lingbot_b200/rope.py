@@ -28,32 +28,33 @@ class Rope:
 
     def __post_init__(self):
         c, s = self.cos, self.sin
-        if c.dtype != torch.float32 or s.dtype != torch.float32 or c.dim() != 2 or c.shape != s.shape \
-                or c.stride() != s.stride() or c.stride(1) != 1 or c.device != s.device:
+        if not (c.dtype == s.dtype == torch.float32 and c.dim() == 2 and c.shape == s.shape and c.stride() == s.stride()
+                and c.stride(1) == 1 and c.device == s.device):
             raise ValueError("rope tables: two float32 [positions, rot / 2] tensors of one device and layout with unit "
                              f"last stride, got {c.dtype} {tuple(c.shape)} and {s.dtype} {tuple(s.shape)}")
         if not c.is_cuda:
             raise ValueError("rope tables must be CUDA tensors")
+        rows, half = c.shape
+        self.rot = 2 * half
+        self._args = (c.data_ptr(), s.data_ptr(), c.stride(0), rows, 2 * half, int(self.interleaved))
 
-    @property
-    def rot(self):
-        return 2 * self.cos.shape[1]
-
-    def args(self, positions, device, shape):
-        """The table and position arguments of the C ABI, for tokens of `shape` [B, L]."""
+    def args(self, positions, device, b, l):
+        """The table and position arguments of the C ABI, for tokens [b, l]."""
         if self.cos.device != device:
             raise ValueError(f"rope tables on {self.cos.device}, tensors on {device}")
-        pos, pos64, sb, sl = None, 0, 0, 0
-        if positions is not None:
-            if positions.dtype not in _POS or positions.device != device:
-                raise TypeError("positions must be an int32 or int64 tensor on the tensors' device")
-            p = positions if positions.dim() == 2 else positions[None]
-            if p.dim() != 2 or p.shape[1] != shape[1] or p.shape[0] not in (1, shape[0]):
-                raise ValueError(f"positions {tuple(positions.shape)} for tokens {tuple(shape)}")
-            pos, pos64 = p.data_ptr(), int(p.dtype == torch.int64)
-            sb, sl = (p.stride(0) if p.shape[0] > 1 else 0), p.stride(1)
-        return (self.cos.data_ptr(), self.sin.data_ptr(), self.cos.stride(0), self.cos.shape[0], self.rot,
-                int(self.interleaved), pos, pos64, sb, sl)
+        if positions is None:
+            return (*self._args, None, 0, 0, 0)
+        dt = positions.dtype
+        if dt not in _POS or positions.device != device:
+            raise TypeError("positions must be an int32 or int64 tensor on the tensors' device")
+        shape = tuple(positions.shape)
+        if shape == (b, l):
+            sb, sl = positions.stride()
+        elif shape == (l,) or shape == (1, l):
+            sb, sl = 0, positions.stride(-1)
+        else:
+            raise ValueError(f"positions {shape} for tokens {(b, l)}")
+        return (*self._args, positions.data_ptr(), 1 if dt is torch.int64 else 0, sb, sl)
 
 
 def tables(num_positions, rot, base=10000.0, scaling=None, device="cuda", interleaved=True) -> Rope:
@@ -102,10 +103,7 @@ def _check(name, x):
         raise ValueError(f"{name} must be [B, L, heads, dim] with unit channel stride, got {tuple(x.shape)}")
 
 
-def _output(name, x, out):
-    """The tensor that takes x's result: `out` (x itself for in place), or a new one."""
-    if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+def _check_out(name, x, out):
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (out.numel() and out.stride(3) != 1):
         raise ValueError(f"{name} out: {out.dtype} {tuple(out.shape)} does not match {x.dtype} {tuple(x.shape)}")
     same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
@@ -113,7 +111,6 @@ def _output(name, x, out):
         raise ValueError(f"{name} out shares memory with its input without being it")
     if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
         raise ValueError(f"{name} out has elements that share memory")
-    return out
 
 
 def apply(x, rope: Rope, positions=None, start=0, inverse=False, out=None, k=None, k_out=None):
@@ -123,26 +120,41 @@ def apply(x, rope: Rope, positions=None, start=0, inverse=False, out=None, k=Non
     place. inverse=True turns back: apply(grad, ..., inverse=True) is the gradient."""
     _check("x", x)
     b, l, h, d = x.shape
-    if torch.is_grad_enabled() and (x.requires_grad or (k is not None and k.requires_grad)):
-        raise RuntimeError("rope.apply records no gradient: call it under torch.no_grad(), and rotate the gradient back "
-                           "with inverse=True")
-    y = _output("x", x, out)
-    k_args, y2 = (None, 0, 0, 0, None, 0, 0, 0, 0), None
-    if k is not None:
-        _check("k", k)
-        if k.shape[:2] != x.shape[:2] or k.shape[3] != d or k.dtype != x.dtype or k.device != x.device:
-            raise ValueError(f"k {k.dtype} {tuple(k.shape)} does not go with x {x.dtype} {tuple(x.shape)}")
-        y2 = _output("k", k, k_out)
-        if (out is None) != (k_out is None):
-            raise ValueError("out and k_out: give both or neither")
-        if h and k.numel() and (y.data_ptr() == k.data_ptr() or y2.data_ptr() == x.data_ptr()):
+    dev = x.device
+    if x.requires_grad or (k is not None and k.requires_grad):
+        if torch.is_grad_enabled():
+            raise RuntimeError("rope.apply records no gradient: call it under torch.no_grad(), and rotate the gradient "
+                               "back with inverse=True")
+    if (out is None) != (k_out is None) and k is not None:
+        raise ValueError("out and k_out: give both or neither")
+    if out is None:
+        y = torch.empty_like(x)
+    else:
+        _check_out("x", x, out)
+        y = out
+    sx, sy = x.stride(), y.stride()
+    table = rope.args(positions, dev, b, l)
+    if k is None:
+        if b and l and h:
+            _lib.call_on(dev, "lbq_rope", x.data_ptr(), sx[0], sx[1], sx[2], y.data_ptr(), sy[0], sy[1], sy[2], h, None, 0, 0,
+                         0, None, 0, 0, 0, 0, b, l, d, *table, int(start), 1 if inverse else 0, _DTYPES[x.dtype])
+        return y
+    _check("k", k)
+    kb, kl, hk, kd = k.shape
+    if kb != b or kl != l or kd != d or k.dtype != x.dtype or k.device != dev:
+        raise ValueError(f"k {k.dtype} {tuple(k.shape)} does not go with x {x.dtype} {tuple(x.shape)}")
+    if k_out is None:
+        z = torch.empty_like(k)
+    else:
+        _check_out("k", k, k_out)
+        z = k_out
+        if h and hk and (y.data_ptr() == k.data_ptr() or z.data_ptr() == x.data_ptr()):
             raise ValueError("out and k_out are swapped: each is written while the other's input is read")
-        if k.shape[2]:
-            k_args = (k.data_ptr(), *k.stride()[:3], y2.data_ptr(), *y2.stride()[:3], k.shape[2])
-    table = rope.args(positions, x.device, (b, l))
-    if b and l and h:
-        _lib.call_on(x.device, "lbq_rope", x.data_ptr(), *x.stride()[:3], y.data_ptr(), *y.stride()[:3], h, *k_args, b, l,
-                     d, *table, int(start), int(bool(inverse)), _DTYPES[x.dtype])
-    elif k is not None and b and l and k.shape[2]:
-        raise ValueError("x has no heads: rotate k alone")
-    return y if k is None else (y, y2)
+    if not (h and hk):
+        raise ValueError(f"x with {h} heads and k with {hk}: rotate the one that has heads alone")
+    if b and l:
+        sk, sz = k.stride(), z.stride()
+        _lib.call_on(dev, "lbq_rope", x.data_ptr(), sx[0], sx[1], sx[2], y.data_ptr(), sy[0], sy[1], sy[2], h, k.data_ptr(),
+                     sk[0], sk[1], sk[2], z.data_ptr(), sz[0], sz[1], sz[2], hk, b, l, d, *table, int(start),
+                     1 if inverse else 0, _DTYPES[x.dtype])
+    return y, z
