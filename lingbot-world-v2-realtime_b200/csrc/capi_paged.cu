@@ -77,7 +77,7 @@ int finish(cudaError_t e, const char* what) {
 // Query rows (token, query head of the K/V head) that one CTA takes, by the rows of a K/V head: the few-row kernel up
 // to kFewRows, the many-row kernel above.
 constexpr int64_t kFewRows = 64;
-int attn_tile_rows(int64_t rows) { return rows <= kFewRows ? lbq::kFewTile : lbq::kManyTile; }
+int attn_tile_rows(int64_t rows) { return rows <= 8 ? 8 : (rows <= kFewRows ? 16 : lbq::kManyTile); }
 
 }  // namespace
 
@@ -264,8 +264,8 @@ int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t ma
   const int64_t pages = (max_kv_len + lbq::kPageTokens - 1) / lbq::kPageTokens;
   // few rows: two CTAs an SM, a split keeps at least 4 pages, one for each warp; many rows: one CTA an SM, at least
   // 8 pages (4 key tiles) to pay for the query tiles
-  int64_t n = (tile == lbq::kFewTile ? 2 * 148 : 148) / ctas;
-  const int64_t least = tile == lbq::kFewTile ? 4 : 8;
+  int64_t n = (tile != lbq::kManyTile ? 2 * 148 : 148) / ctas;
+  const int64_t least = tile != lbq::kManyTile ? 4 : 8;
   if (n > pages / least) n = pages / least;
   return int(n < 1 ? 1 : (n > 1024 ? 1024 : n));
 }
@@ -349,7 +349,7 @@ int lbq_paged_attn(const void* q, int64_t sq_b, int64_t sq_l, int64_t sq_h, cons
   a.v_unit = 1.f / lbq::code_max(fmt);
   a.status = lbq::device_status_ptr();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a.tile_rows == lbq::kFewTile) {
+  if (a.tile_rows != lbq::kManyTile) {
     CUtensorMap tk, tv;
     const uint64_t prows = uint64_t(num_pages) * heads * lbq::kPageTokens;
     if ((r = lbq::make_page_map(&tk, k_pages, prows, "k_pages", lbq::kPageTokens)) ||

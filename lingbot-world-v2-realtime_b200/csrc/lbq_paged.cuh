@@ -8,6 +8,10 @@
 
 namespace lbq {
 
+constexpr float kTinyScale = 5.421010862427522e-20f;   // 2^-64: scales are kept above it (a written page's are >= 2^-40)
+constexpr float kWeightBits = 7.f;               // weights are scaled by 2^7 ...
+constexpr float kSlack = 8.f;                    // ... and the running maximum may lag by 2^8: below 2^15, fp16's range
+
 // Keys [0, visible) are seen by some row of the tile; 0 when every row is empty or past the sequence's queries.
 struct TileKeys {
   int64_t kv;

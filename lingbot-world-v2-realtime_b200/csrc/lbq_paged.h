@@ -77,7 +77,7 @@ struct PageReadArgs {
   int* status;
 };
 
-constexpr int kFewTile = 16, kManyTile = 256;   // query rows of a CTA: few-row and many-row attention kernels
+constexpr int kManyTile = 256;                  // query rows of a CTA of the many-row attention kernel
 
 constexpr int kCopyPairs = 480;               // page pairs of one launch (they travel as kernel parameters)
 struct PageCopyArgs {

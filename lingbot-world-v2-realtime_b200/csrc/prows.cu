@@ -41,10 +41,6 @@ constexpr int kTile16 = 2 * kHalf;               // a 128 x 128 fp16 tile
 constexpr int kRowStages = 2;
 constexpr uint32_t kRegSoftmax = 168, kRegWiden = 128, kRegIssue = 48;
 static_assert(128 * (2 * kRegSoftmax + kRegWiden + kRegIssue) <= kRowThreads * 128, "register split");
-constexpr float kTinyScale = 5.421010862427522e-20f;   // 2^-64
-constexpr float kWeightBits = 7.f;               // weights are scaled by 2^7 ...
-constexpr float kSlack = 8.f;                    // ... and the running maximum may lag by 2^8: below 2^15, fp16's range
-
 struct RowsShared {
   uint64_t q_full;                               // both query tiles in shared memory (256 threads)
   uint64_t k_full[kRowStages], v_full[kRowStages];      // 128 widening threads
@@ -121,6 +117,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
   uint8_t* sV = sK + kRowStages * kTile16;
   RowsShared* sh = reinterpret_cast<RowsShared*>(sV + kRowStages * kTile16);
   volatile int* abort_flag = &sh->abort;
+  asm volatile("griddepcontrol.launch_dependents;");     // a merge of key splits may be launched; it waits for the end
   // the last row tiles see the most keys under a causal mask: they start first
   const int tile = a.tiles - 1 - int(blockIdx.x % a.tiles), h = blockIdx.x / a.tiles, split = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

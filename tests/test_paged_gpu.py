@@ -212,6 +212,17 @@ def test_attend_key_splits(splits, lq, group):
     run_attend(q, pages, table, kvs, [lq] * 4, True, num_splits=splits)
 
 
+@pytest.mark.parametrize("lq,group", [(1, 1), (3, 5), (90, 1)])
+def test_attend_long_splits(lq, group):
+    """Hundreds of pages in one split: the ring of page slots goes round many times in every warp's order."""
+    kvs = [20000, 12345]
+    pages = P.make_pages(12, 510, 1, torch.int8)
+    table = P.make_table(5, [313, 193], 510)
+    q = torch.randn(2, lq, group, 128, generator=torch.Generator().manual_seed(1)).bfloat16()
+    outs = [run_attend(q, pages, table, kvs, [lq] * 2, True, num_splits=n)[0] for n in (1, 1, 1, 4)]
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
 @FORMATS
 @pytest.mark.parametrize("lq", [1, 129], ids=["token", "chunk"])
 def test_attend_wide_ranges(fmt, lq):
