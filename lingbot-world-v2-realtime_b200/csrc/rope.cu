@@ -69,6 +69,8 @@ __device__ __forceinline__ void store_n(typename ActType<kDt>::T* p, const float
   }
 }
 
+constexpr int kBatch = 2;
+
 // Block (units, heads in flight): unit u of a head is kN channels (interleaved) or kN pairs (half) of the rotated
 // part, or kN channels of the rest, which is copied unless the call is in place.
 template <int kDt, bool kInter, int kN>
@@ -102,34 +104,47 @@ __global__ void rope_kernel(const RopeArgs a) {
   }
   const int heads = a.heads[0] + a.heads[1];
   const int ch = turn ? u * kN : a.rope.rot + (u - rot_units) * kN;
-  for (int hh = threadIdx.y; hh < heads; hh += blockDim.y) {
-    const int w = hh >= a.heads[0];
-    const int h = w ? hh - a.heads[0] : hh;
-    const T* x = static_cast<const T*>(a.x[w]) + b * a.sx[w][0] + l * a.sx[w][1] + h * a.sx[w][2] + ch;
-    T* y = static_cast<T*>(a.y[w]) + b * a.sy[w][0] + l * a.sy[w][1] + h * a.sy[w][2] + ch;
-    float f[kN];
-    load_n<kDt, kN>(x, f);
-    if (!turn) {
-      store_n<kDt, kN>(y, f);
-    } else if constexpr (kInter) {
+  // kBatch heads at a time, all their loads first: one head a thread leaves too few bytes in flight (4.5 TB/s on 6032
+  // tokens of 24 heads)
+  for (int h0 = threadIdx.y; h0 < heads; h0 += kBatch * blockDim.y) {
+    const T* x[kBatch];
+    T* y[kBatch];
+    float f[kBatch][kN], g[kBatch][kInter ? 1 : kN];
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        const float p = f[2 * i], q = f[2 * i + 1];
-        f[2 * i] = __fsub_rn(__fmul_rn(p, c[i]), __fmul_rn(q, s[i]));
-        f[2 * i + 1] = __fadd_rn(__fmul_rn(p, s[i]), __fmul_rn(q, c[i]));
+    for (int k = 0; k < kBatch; ++k) {
+      const int hh = h0 + k * blockDim.y;
+      if (hh >= heads) break;
+      const int w = hh >= a.heads[0];
+      const int h = w ? hh - a.heads[0] : hh;
+      x[k] = static_cast<const T*>(a.x[w]) + b * a.sx[w][0] + l * a.sx[w][1] + h * a.sx[w][2] + ch;
+      y[k] = static_cast<T*>(a.y[w]) + b * a.sy[w][0] + l * a.sy[w][1] + h * a.sy[w][2] + ch;
+      load_n<kDt, kN>(x[k], f[k]);
+      if constexpr (!kInter) {
+        if (turn) load_n<kDt, kN>(x[k] + a.rope.rot / 2, g[k]);
       }
-      store_n<kDt, kN>(y, f);
-    } else {
-      float g[kN];
-      load_n<kDt, kN>(x + a.rope.rot / 2, g);
+    }
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const float p = f[i], q = g[i];
-        f[i] = __fsub_rn(__fmul_rn(p, c[i]), __fmul_rn(q, s[i]));
-        g[i] = __fadd_rn(__fmul_rn(p, s[i]), __fmul_rn(q, c[i]));
+    for (int k = 0; k < kBatch; ++k) {
+      if (h0 + k * int(blockDim.y) >= heads) break;
+      if (turn) {
+        if constexpr (kInter) {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            const float p = f[k][2 * i], q = f[k][2 * i + 1];
+            f[k][2 * i] = __fsub_rn(__fmul_rn(p, c[i]), __fmul_rn(q, s[i]));
+            f[k][2 * i + 1] = __fadd_rn(__fmul_rn(p, s[i]), __fmul_rn(q, c[i]));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const float p = f[k][i], q = g[k][i];
+            f[k][i] = __fsub_rn(__fmul_rn(p, c[i]), __fmul_rn(q, s[i]));
+            g[k][i] = __fadd_rn(__fmul_rn(p, s[i]), __fmul_rn(q, c[i]));
+          }
+          store_n<kDt, kN>(y[k] + a.rope.rot / 2, g[k]);
+        }
       }
-      store_n<kDt, kN>(y, f);
-      store_n<kDt, kN>(y + a.rope.rot / 2, g);
+      store_n<kDt, kN>(y[k], f[k]);
     }
   }
 }

@@ -80,6 +80,7 @@ SIGNATURES = {
 _lock = threading.Lock()
 _lib = None
 _entry = {}
+_fast = None
 
 
 class LbqError(RuntimeError):
@@ -106,6 +107,30 @@ def load():
     return _lib
 
 
+def fast():
+    """The calls straight from torch tensors (_torchcall), bound to the loaded library's entries. They return None where
+    a call is not of the usual form, else their result or an entry's status code."""
+    global _fast
+    if _fast is None:
+        lib = load()
+        try:
+            from . import _torchcall
+        except ImportError as e:
+            raise ImportError("lingbot_b200/_torchcall.so is missing or does not load: build it with `python -m "
+                              f"lingbot_b200.build` ({e})") from e
+        _torchcall.init(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in
+                          ("lbq_rope", "lbq_page_write", "lbq_page_read", "lbq_paged_attn", "lbq_paged_attn_splits",
+                           "lbq_paged_attn_workspace")))
+        _fast = _torchcall
+    return _fast
+
+
+def check(name, rc):
+    """Raise LbqError for a status code other than 0."""
+    if rc != 0:
+        raise LbqError(f"{name} failed ({rc}): {_lib.lbq_last_error().decode(errors='replace')}")
+
+
 def call(name, *args):
     """Call an lbq_* entry point that returns a status code; raise LbqError on failure."""
     lib = load()
@@ -128,8 +153,7 @@ def call_on(device, name, *args):
     else:
         with torch.cuda.device(device):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc != 0:
-        raise LbqError(f"{name} failed ({rc}): {_lib.lbq_last_error().decode(errors='replace')}")
+    check(name, rc)
 
 
 def device_status(clear=True):

@@ -16,6 +16,10 @@ SOURCES = ["quant.cu", "attn.cu", "fp8lin.cu", "capi.cu", "noalloc.cu", "peer.cu
 HEADERS = ["lbq_ptx.cuh", "lbq_kernels.h", "lbq_peer.cuh", "lbq_paged.h", "lbq_paged.cuh", os.path.join("..", "..", "include", "lbq.h")]
 
 
+BINDING = os.path.join(PKG_DIR, "_torchcall.so")
+BINDING_DEPS = ["torchcall.cpp", os.path.join("..", "..", "include", "lbq.h")]
+
+
 def nvcc():
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     path = os.path.join(cuda, "bin", "nvcc")
@@ -37,12 +41,37 @@ def stale(lib=None):
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def build_binding(force=False, verbose=False):
+    """Compile _torchcall.so, the calls of the paged-cache and rotary entries straight from torch tensors (host code
+    against torch's headers). Returns its path."""
+    deps = [os.path.join(CSRC, d) for d in BINDING_DEPS]
+    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
+        return BINDING
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in inc),
+           os.path.join(CSRC, "torchcall.cpp"), "-o", BINDING + ".tmp", "-L" + os.path.join(root, "lib"), "-lc10",
+           "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(BINDING + ".tmp", BINDING)
+    return BINDING
+
+
 def build(force=False, verbose=False, extra=(), debug=False):
     """Compile each .cu to an object, then link the shared library. Returns the library path.
     debug=True builds liblbq_debug.so instead: the same kernels with the device-side index checks
     (-DLBQ_DEBUG=1) that record a 0x3xx status code where the index arithmetic goes wrong; the
     package loads it when LBQ_DEBUG_LIB=1."""
     lib = DEBUG_LIB if debug else LIB
+    build_binding(force and not debug, verbose)
     if not force and not stale(lib):
         return lib
     objs = []

@@ -55,6 +55,7 @@ class Pages:
         if not k.is_cuda or v.device != dev or ka.device != dev or va.device != dev:
             raise ValueError("pages must be CUDA tensors of one device")
         self.device = dev
+        self._dev = k.get_device()
         self.heads = k.shape[-3]
         self._args = None if k.dim() == 5 else (k.data_ptr(), ka.data_ptr(), v.data_ptr(), va.data_ptr(), k.shape[0],
                                                 self.heads, FORMATS[k.dtype])
@@ -127,6 +128,12 @@ def write(pages: Pages, page_table, start, k, v, lens=None, rope: Rope = None, p
     keeps them: when its largest magnitude grows their codes are rounded to the new scale. Tokens at and past `start`
     are replaced. With `rope`, K is rotated on the way, by `positions` [B, L] or its token indices, to the same bits as
     rope.apply followed by a plain write. Two sequences of one call must not write the same page."""
+    if rope is None or rope._dev == pages._dev:
+        r = _lib.fast().page_write(pages._args, pages._dev, page_table, start, k, v, lens, None if rope is None else rope._args,
+                                   positions)
+        if r is not None:
+            _lib.check("lbq_page_write", r)
+            return
     args, heads, dev = pages.args(), pages.heads, pages.device
     _check_rows("k", k, dev)
     _check_rows("v", v, dev)
@@ -165,6 +172,12 @@ def write(pages: Pages, page_table, start, k, v, lens=None, rope: Rope = None, p
 def window(pages: Pages, page_table, start, length, dtype=torch.bfloat16, lens=None, out=None):
     """Values (k, v) [B, length, heads, 128] in `dtype` of the tokens from start[b] on; rows past lens[b] (None: all) are
     0. The role of kv_cache.window, as a copy."""
+    if out is None and dtype in _ACT:
+        r = _lib.fast().page_read(pages._args, pages._dev, page_table, start, length, _ACT[dtype], lens)
+        if r is not None:
+            if type(r) is int:
+                _lib.check("lbq_page_read", r)
+            return r
     args, heads, dev = pages.args(), pages.heads, pages.device
     b, length = page_table.shape[0], int(length)
     if dtype not in _ACT:
@@ -204,6 +217,12 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
     a padded batch. Rows that see no token, and rows past q_lens[b], are 0. Returns out [B, Lq, heads, 128] in q's dtype,
     with return_lse also the rows' log-sum-exp f32 [B, Lq, heads] (-inf for those rows). max_kv_len bounds kv_lens where
     the page table is much wider than the longest sequence; num_splits overrides the number of key splits."""
+    if out is None and not return_lse and max_kv_len is None and num_splits is None:
+        r = _lib.fast().paged_attn(pages._args, pages._dev, q, page_table, kv_lens, q_lens, causal, float(sm_scale or 0.0))
+        if r is not None:
+            if type(r) is int:
+                _lib.check("lbq_paged_attn", r)
+            return r
     args, heads, dev = pages.args(), pages.heads, pages.device
     _check_rows("q", q, dev)
     b, lq, hq, _ = q.shape

@@ -36,6 +36,7 @@ class Rope:
             raise ValueError("rope tables must be CUDA tensors")
         rows, half = c.shape
         self.rot = 2 * half
+        self._dev = c.get_device()
         self._args = (c.data_ptr(), s.data_ptr(), c.stride(0), rows, 2 * half, int(self.interleaved))
 
     def args(self, positions, device, b, l):
@@ -118,6 +119,12 @@ def apply(x, rope: Rope, positions=None, start=0, inverse=False, out=None, k=Non
     unit channel stride) by the table rows `positions` ([B, L] or [L], int32 / int64), or start + l. With `k` (the same
     B, L, dim and dtype, its own heads) both are rotated in one launch, and (x', k') is returned. out=x rotates in
     place. inverse=True turns back: apply(grad, ..., inverse=True) is the gradient."""
+    if out is None and k_out is None:
+        r = _lib.fast().rope(x, k, rope._args, rope._dev, positions, start, inverse)
+        if r is not None:
+            if type(r) is int:
+                _lib.check("lbq_rope", r)
+            return r
     _check("x", x)
     b, l, h, d = x.shape
     dev = x.device
