@@ -96,7 +96,6 @@ int lbq_rope(const void* x, int64_t sx_b, int64_t sx_l, int64_t sx_h, void* y, i
   if (heads <= 0 || heads > kMaxGrid || heads2 < 0 || heads2 > kMaxGrid) return set_error(LBQ_ERR_ARG, "heads out of range");
   if ((r = check_batch(batch, len, "len"))) return r;
   if (dim <= 0 || dim > 512 || dim % 2) return set_error(LBQ_ERR_ARG, "dim %d must be even and in [2, 512]", dim);
-  if (int64_t(batch) * len > (int64_t(1) << 31) - 1) return set_error(LBQ_ERR_ARG, "too many tokens");
   const int size = dtype == 2 ? 4 : 2;
   const void* ptrs[4] = {x, y, x2, y2};
   const int64_t strides[4][3] = {{sx_b, sx_l, sx_h}, {sy_b, sy_l, sy_h}, {sx2_b, sx2_l, sx2_h}, {sy2_b, sy2_l, sy2_h}};
@@ -117,6 +116,7 @@ int lbq_rope(const void* x, int64_t sx_b, int64_t sx_l, int64_t sx_h, void* y, i
   const int vec = 16 / size;
   // 16-byte accesses where a 16-byte piece lies wholly in the rotated part (or in one half of it) or in the rest
   a.vec = wide && rot % (interleaved ? vec : 2 * vec) == 0 && (dim - rot) % vec == 0;
+  a.wide_table = rope_stride % 4 == 0 && aligned(rope_cos, 16) && aligned(rope_sin, 16);
   for (int i = 0; i < 2; ++i) {
     a.x[i] = i ? x2 : x;
     a.y[i] = i ? y2 : y;

@@ -44,6 +44,7 @@ struct RopeArgs {
   int batch, len, dim;
   int dtype;                    // 0 bf16, 1 fp16, 2 fp32
   int vec;                      // 16-byte accesses
+  int wide_table;               // the tables' rows are 16-byte aligned
   int inverse;
   int64_t start;                // position of token 0 when the table has no `pos`
   RopeTable rope;

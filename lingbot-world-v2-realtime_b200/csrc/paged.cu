@@ -16,6 +16,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "lbq_kernels.h"
 #include "lbq_paged.h"
@@ -81,50 +82,56 @@ __device__ __forceinline__ uint4 pack_act8(const float (&f)[8]) {
                     pack_act2(f[6], f[7], kDt));
 }
 
-// Rotates the 8 channels 8 * c16 .. of one K row (rope.cu's arithmetic: products and sums rounded one by one, the
-// result rounded to the activation type). `row`: the head's 128 channels in memory, for the half layout's partners.
-template <int kDt>
-__device__ __forceinline__ uint4 rope_row8(const uint4 raw, const uint16_t* row, int c16, const RopeTable& r,
-                                           int64_t at) {
+// One thread's part of a table row: the cosines and sines of its 8 channels (4 pairs of neighbours, or 8 pairs whose other
+// half another thread holds).
+template <int kRope>
+struct Turn {
+  static constexpr int kN = kRope == 2 ? 8 : 4;
+  float4 c[kN / 4], s[kN / 4];
+  __device__ __forceinline__ void load(const float* cs, const float* sn) {
+#pragma unroll
+    for (int i = 0; i < kN / 4; ++i) {
+      c[i] = reinterpret_cast<const float4*>(cs)[i];
+      s[i] = reinterpret_cast<const float4*>(sn)[i];
+    }
+  }
+};
+// Rotates 8 channels (rope.cu's arithmetic: products and sums rounded one by one, the result rounded to the activation
+// type). `other`: the same channels of the pairs' other half, `low`: x is the first half (half layout).
+template <int kDt, int kRope>
+__device__ __forceinline__ uint4 rotate8(const uint4 raw, const uint4 other, bool low, const Turn<kRope>& t) {
   float x[8];
   unpack_act8<kDt>(raw, x);
-  const int ch = c16 * 8, half = r.rot / 2;
-  if (r.interleaved) {
-    const float4 c = *reinterpret_cast<const float4*>(r.cos + at * r.stride + ch / 2);
-    const float4 s = *reinterpret_cast<const float4*>(r.sin + at * r.stride + ch / 2);
-    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+  if constexpr (kRope == 1) {
+    const float c[4] = {t.c[0].x, t.c[0].y, t.c[0].z, t.c[0].w}, s[4] = {t.s[0].x, t.s[0].y, t.s[0].z, t.s[0].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float p = x[2 * i], q = x[2 * i + 1];
-      x[2 * i] = __fsub_rn(__fmul_rn(p, cc[i]), __fmul_rn(q, ss[i]));
-      x[2 * i + 1] = __fadd_rn(__fmul_rn(p, ss[i]), __fmul_rn(q, cc[i]));
+      x[2 * i] = __fsub_rn(__fmul_rn(p, c[i]), __fmul_rn(q, s[i]));
+      x[2 * i + 1] = __fadd_rn(__fmul_rn(p, s[i]), __fmul_rn(q, c[i]));
     }
   } else {
-    const bool low = ch < half;
-    const int k0 = low ? ch : ch - half;
     float o[8];
-    unpack_act8<kDt>(*reinterpret_cast<const uint4*>(row + (low ? ch + half : ch - half)), o);
+    unpack_act8<kDt>(other, o);
 #pragma unroll
-    for (int q4 = 0; q4 < 2; ++q4) {
-      const float4 c = *reinterpret_cast<const float4*>(r.cos + at * r.stride + k0 + 4 * q4);
-      const float4 s = *reinterpret_cast<const float4*>(r.sin + at * r.stride + k0 + 4 * q4);
-      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 4 * q4 + i;
-        x[j] = low ? __fsub_rn(__fmul_rn(x[j], cc[i]), __fmul_rn(o[j], ss[i]))
-                   : __fadd_rn(__fmul_rn(o[j], ss[i]), __fmul_rn(x[j], cc[i]));
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float4 cv = t.c[i >> 2], sv = t.s[i >> 2];
+      const float c = (i & 3) == 0 ? cv.x : (i & 3) == 1 ? cv.y : (i & 3) == 2 ? cv.z : cv.w;
+      const float s = (i & 3) == 0 ? sv.x : (i & 3) == 1 ? sv.y : (i & 3) == 2 ? sv.z : sv.w;
+      // the first half x c - o s, the second o s + x c: one sign apart, and a sum of two products commutes
+      const float os = __fmul_rn(o[i], s);
+      x[i] = __fadd_rn(__fmul_rn(x[i], c), low ? -os : os);
     }
   }
   return pack_act8<kDt>(x);
 }
 
 // The codes of one thread's rows by IEEE divisions, for any scale and any value; kept out of line, away from the
-// registers and the instruction stream of the usual path.
+// registers and the instruction stream of the usual path (and given its rows by value: a reference would put them in local
+// memory, 64 bytes a thread written and read for nothing).
 template <int kFmt, int kDt>
-__device__ __noinline__ void general_codes(const uint4 (&raw)[4], uint8_t* codes, int rg, int c16, int lo, int hi, float amax,
-                                           float old) {
+__device__ __noinline__ void general_codes(uint4 r0, uint4 r1, uint4 r2, uint4 r3, uint8_t* codes, int rg, int c16, int lo,
+                                           int hi, float amax, float old) {
   constexpr float kQ = kFmt ? 448.f : 127.f;
   // both operands scaled by 2^-64 where x * Q could overflow
   const float f = amax > 1.8446744073709552e19f ? 5.421010862427522e-20f : 1.f;      // 2^64, 2^-64
@@ -134,7 +141,7 @@ __device__ __noinline__ void general_codes(const uint4 (&raw)[4], uint8_t* codes
     uint2* dst = reinterpret_cast<uint2*>(codes + r * 128 + c16 * 8);
     float x[8];
     if (r >= lo && r < hi) {
-      unpack_act8<kDt>(raw[i], x);
+      unpack_act8<kDt>(i == 0 ? r0 : i == 1 ? r1 : i == 2 ? r2 : r3, x);
       for (int j = 0; j < 8; ++j) {
         const float v = x[j] != x[j] ? 0.f : fminf(fmaxf(x[j], -amax), amax);
         x[j] = __fdiv_rn(__fmul_rn(v, f * kQ), amax * f);
@@ -155,61 +162,75 @@ __device__ __noinline__ void general_codes(const uint4 (&raw)[4], uint8_t* codes
   }
 }
 
-// One CTA per (touched page, head, sequence) and tensor (grid.x even: K, odd: V). 256 threads = 16 chunks of 8
-// channels x 16 row groups; a thread takes rows rg + 16 i. The new rows stay in registers between the maximum and
-// the codes, so each value is read once.
-template <int kFmt, int kDt>
-__global__ void __launch_bounds__(256) page_write_kernel(const PageWriteArgs a) {
-  const int w = blockIdx.x & 1, h = blockIdx.y, b = blockIdx.z;
+// One CTA per (touched page, head, sequence) and tensor. 256 threads = 16 chunks of 8 channels x 16 row groups; a thread
+// takes rows rg + 16 i. The new rows stay in registers between the maximum and the codes, so each value is read once; all
+// loads go out before the page is looked up.
+template <int kFmt, int kDt, int kRope>
+__device__ __forceinline__ void write_page(const PageWriteArgs& a, const int w, uint32_t* red) {
+  const int h = blockIdx.y, b = blockIdx.z;
   const int t = threadIdx.x, c16 = t & 15, rg = t >> 4;
   const int64_t start = a.start ? a.start[b] : a.start0;
   int n = a.lens ? a.lens[b] : a.len;
   n = n < 0 ? 0 : (n > a.len ? a.len : n);
-  const int64_t blk = start / kPageTokens + (blockIdx.x >> 1);
-  const int64_t t0 = blk * kPageTokens;
-  const int lo = int(start > t0 ? start - t0 : 0);                       // rows held before
-  const int64_t end = start + n - t0;
-  const int hi = int(end < kPageTokens ? end : kPageTokens);             // rows [lo, hi) are new
   if (start < 0) {
     if (a.status && t == 0) atomicCAS(a.status, 0, kDevBadPage);
     return;
   }
+  const int off = int(start % kPageTokens);                              // the first touched page's held rows
+  const int l0 = int(blockIdx.x >> 1) * kPageTokens - off;               // source row of this page's row 0
+  const int lo = l0 < 0 ? -l0 : 0, hi = min(n - l0, kPageTokens);        // rows [lo, hi) are new
   if (hi <= lo) return;
-  const int64_t* ss = a.ss[w];
-  const uint16_t* src = static_cast<const uint16_t*>(a.src[w]) + b * ss[0] + h * ss[2];
-  const bool rope = w == 0 && a.rope.cos != nullptr && c16 * 8 < a.rope.rot;
-  // rows outside [lo, hi) load a neighbour's, so that no load waits for a branch, and count as 0
+  const int64_t blk = start / kPageTokens + (blockIdx.x >> 1);
+  const int64_t sl = a.ss[w][1];
+  const uint16_t* src = static_cast<const uint16_t*>(a.src[w]) + b * a.ss[w][0] + h * a.ss[w][2] + (l0 + rg) * sl + c16 * 8;
   uint4 raw[4];
-  int64_t at[4];
+  bool on[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t l = t0 + min(max(rg + 16 * i, lo), hi - 1) - start;
-    raw[i] = *reinterpret_cast<const uint4*>(src + l * ss[1] + c16 * 8);
-    at[i] = start + l;
-    if (rope && a.rope.pos != nullptr) {
-      const int64_t o = b * a.rope.sp_b + l * a.rope.sp_l;
-      at[i] = a.rope.pos64 ? static_cast<const int64_t*>(a.rope.pos)[o] : static_cast<const int32_t*>(a.rope.pos)[o];
-    }
+    on[i] = rg + 16 * i >= lo && rg + 16 * i < hi;
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (on[i]) raw[i] = *reinterpret_cast<const uint4*>(src + 16 * i * sl);
   }
   const int page = page_of(a.pt, b, blk, a.status);
+  if constexpr (kRope != 0) {
+    if (c16 * 8 < a.rope.rot) {
+      const int half = a.rope.rot / 2, ch = c16 * 8;
+      const bool low = kRope == 1 || ch < half;
+      const int col = kRope == 1 ? ch / 2 : (low ? ch : ch - half);
+#pragma unroll
+      for (int i2 = 0; i2 < 4; i2 += 2) {                                // two rows at a time
+        Turn<kRope> turn[2];
+        uint4 other[2];
+        bool in[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int i = i2 + k, l = l0 + rg + 16 * i;
+          int64_t at = start + l;
+          in[k] = false;
+          if (on[i]) {
+            if (a.rope.pos != nullptr) {
+              const int64_t o = b * a.rope.sp_b + l * a.rope.sp_l;
+              at = a.rope.pos64 ? static_cast<const int64_t*>(a.rope.pos)[o] : static_cast<const int32_t*>(a.rope.pos)[o];
+            }
+            in[k] = at >= 0 && at < a.rope.rows;
+            if (!in[k] && a.status) atomicCAS(a.status, 0, kDevBadPosition);
+          }
+          if (in[k]) {
+            turn[k].load(a.rope.cos + at * a.rope.stride + col, a.rope.sin + at * a.rope.stride + col);
+            if (kRope == 2) other[k] = *reinterpret_cast<const uint4*>(src + 16 * i * sl + (low ? half : -half));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (in[k]) raw[i2 + k] = rotate8<kDt, kRope>(raw[i2 + k], other[k], low, turn[k]);
+      }
+    }
+  }
   if (page < 0) return;
   const int64_t ph = int64_t(page) * a.heads + h;
   uint8_t* codes = a.codes[w] + ph * kPageBytes;
   float* amax_p = a.amax[w] + ph;
   const float old = lo > 0 ? *amax_p : 0.f;
-  if (rope) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool in = at[i] >= 0 && at[i] < a.rope.rows;
-      if (!in && a.status) atomicCAS(a.status, 0, kDevBadPosition);
-      const int64_t l = t0 + min(max(rg + 16 * i, lo), hi - 1) - start;
-      const uint4 turned = rope_row8<kDt>(raw[i], src + l * ss[1], c16, a.rope, in ? at[i] : 0);
-      if (in) raw[i] = turned;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (rg + 16 * i < lo || rg + 16 * i >= hi) raw[i] = make_uint4(0u, 0u, 0u, 0u);
   // largest magnitude, two values at a time: as bits, which order like the magnitudes
   uint32_t top2 = 0;
 #pragma unroll
@@ -217,7 +238,6 @@ __global__ void __launch_bounds__(256) page_write_kernel(const PageWriteArgs a) 
     top2 = __vmaxu2(top2, __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu),
                                    __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
   uint32_t top = __reduce_max_sync(0xffffffffu, max(top2 & 0xffffu, top2 >> 16));
-  __shared__ uint32_t red[8];
   if ((t & 31) == 0) red[t >> 5] = top;
   __syncthreads();
 #pragma unroll
@@ -249,22 +269,27 @@ __global__ void __launch_bounds__(256) page_write_kernel(const PageWriteArgs a) 
   // more than 11 significant bits in a scale, or values that are not finite: the general path
   const bool wide = ((__float_as_uint(amax) | __float_as_uint(old)) & 0x1fffu) != 0;
   if (wide || odd) {
-    general_codes<kFmt, kDt>(raw, codes, rg, c16, lo, hi, amax, old);
+    general_codes<kFmt, kDt>(raw[0], raw[1], raw[2], raw[3], codes, rg, c16, lo, hi, amax, old);
     return;
   }
-  const float r_new = __fdiv_rn(kQ, amax), r_old = __fdiv_rn(old, amax);
+  const float r_new = __fdiv_rn(kQ, amax);
+  uint2* dst = reinterpret_cast<uint2*>(codes + rg * 128 + c16 * 8);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = rg + 16 * i;
-    uint2* dst = reinterpret_cast<uint2*>(codes + r * 128 + c16 * 8);
-    if (r >= lo && r < hi) {
+    if (on[i]) {
       float x[8];
       unpack_act8<kDt>(raw[i], x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = quotient(x[j], r_new);
-      *dst = make_uint2(pack_codes<kFmt>(x[0], x[1], x[2], x[3]), pack_codes<kFmt>(x[4], x[5], x[6], x[7]));
-    } else if (r < lo && amax > old) {
-      const uint2 c = *dst;
+      dst[256 * i] = make_uint2(pack_codes<kFmt>(x[0], x[1], x[2], x[3]), pack_codes<kFmt>(x[4], x[5], x[6], x[7]));
+    }
+  }
+  if (lo > 0 && amax > old) {
+    const float r_old = __fdiv_rn(old, amax);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (rg + 16 * i >= lo) break;
+      const uint2 c = dst[256 * i];
       float x[4], y[4];
       unpack_codes<kFmt>(c.x, x);
       unpack_codes<kFmt>(c.y, y);
@@ -273,17 +298,24 @@ __global__ void __launch_bounds__(256) page_write_kernel(const PageWriteArgs a) 
         x[j] = quotient(x[j], r_old);
         y[j] = quotient(y[j], r_old);
       }
-      *dst = make_uint2(pack_codes<kFmt>(x[0], x[1], x[2], x[3]), pack_codes<kFmt>(y[0], y[1], y[2], y[3]));
+      dst[256 * i] = make_uint2(pack_codes<kFmt>(x[0], x[1], x[2], x[3]), pack_codes<kFmt>(y[0], y[1], y[2], y[3]));
     }
   }
 }
+template <int kFmt, int kDt, int kRope>
+__global__ void __launch_bounds__(256) page_write_kernel(const __grid_constant__ PageWriteArgs a) {
+  __shared__ uint32_t red[8];
+  if (blockIdx.x & 1) write_page<kFmt, kDt, 0>(a, 1, red);
+  else write_page<kFmt, kDt, kRope>(a, 0, red);
+}
 
-// One CTA per (64 tokens read, head, sequence), both tensors: 16 codes in, 16 values (two 16-byte stores) out a thread,
-// row and tensor, two rows a thread, all loads before the first store.
+// One CTA per (64 tokens read, head, sequence), both tensors: 8 codes in, 8 values out a thread, row and tensor, so that a
+// half warp writes a whole 256-byte row (16 codes a thread, as two 16-byte stores, would write every 32-byte sector twice);
+// four rows a thread, all loads before the first store.
 template <int kFmt, int kDt>
-__global__ void __launch_bounds__(256) page_read_kernel(const PageReadArgs a) {
+__global__ void __launch_bounds__(256) page_read_kernel(const __grid_constant__ PageReadArgs a) {
   const int h = blockIdx.y, b = blockIdx.z;
-  const int t = threadIdx.x, c8 = t & 7, rg = t >> 3;
+  const int t = threadIdx.x, c16 = t & 15, rg = t >> 4;
   const int64_t start = a.start ? a.start[b] : a.start0;
   int n = a.lens ? a.lens[b] : a.len;
   n = n < 0 ? 0 : (n > a.len ? a.len : n);
@@ -291,44 +323,38 @@ __global__ void __launch_bounds__(256) page_read_kernel(const PageReadArgs a) {
     if (a.status && t == 0) atomicCAS(a.status, 0, kDevBadPage);
     n = 0;
   }
-  uint4 c[2][2];
-  float unit[2][2];
+  const int l0 = int(blockIdx.x) * 64 + rg;
+  uint2 c[4][2];
+  float unit[4][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t l = int64_t(blockIdx.x) * 64 + rg + 32 * i;
-    int page = -1;
+  for (int i = 0; i < 4; ++i) {
+    const int l = l0 + 16 * i;
     const int64_t tok = start + l;
+    int page = -1;
     if (l < n) page = page_of(a.pt, b, tok / kPageTokens, a.status);
     const int64_t ph = int64_t(page < 0 ? 0 : page) * a.heads + h;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      c[i][w] = make_uint4(0u, 0u, 0u, 0u);
+      c[i][w] = make_uint2(0u, 0u);
       unit[i][w] = 0.f;
       if (page >= 0) {
-        c[i][w] = *reinterpret_cast<const uint4*>(a.codes[w] + ph * kPageBytes + (tok % kPageTokens) * 128 + c8 * 16);
+        c[i][w] = *reinterpret_cast<const uint2*>(a.codes[w] + ph * kPageBytes + int(tok % kPageTokens) * 128 + c16 * 8);
         unit[i][w] = a.amax[w][ph];
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t l = int64_t(blockIdx.x) * 64 + rg + 32 * i;
-    if (l >= a.len) break;
+  for (int w = 0; w < 2; ++w) {
+    uint16_t* dst = static_cast<uint16_t*>(a.dst[w]) + b * a.sd[w][0] + l0 * a.sd[w][1] + h * a.sd[w][2] + c16 * 8;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
+    for (int i = 0; i < 4; ++i) {
+      if (l0 + 16 * i >= a.len) break;
       const float u = __fdiv_rn(unit[i][w], kFmt ? 448.f : 127.f);
-      const uint32_t q[4] = {c[i][w].x, c[i][w].y, c[i][w].z, c[i][w].w};
-      uint32_t v[8];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float f[4];
-        unpack_codes<kFmt>(q[k], f);
-        v[2 * k] = pack_act2(f[0] * u, f[1] * u, kDt);
-        v[2 * k + 1] = pack_act2(f[2] * u, f[3] * u, kDt);
-      }
-      uint16_t* dst = static_cast<uint16_t*>(a.dst[w]) + b * a.sd[w][0] + l * a.sd[w][1] + h * a.sd[w][2] + c8 * 16;
-      reinterpret_cast<uint4*>(dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<uint4*>(dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+      float lo[4], hi[4];
+      unpack_codes<kFmt>(c[i][w].x, lo);
+      unpack_codes<kFmt>(c[i][w].y, hi);
+      const float x[8] = {lo[0] * u, lo[1] * u, lo[2] * u, lo[3] * u, hi[0] * u, hi[1] * u, hi[2] * u, hi[3] * u};
+      *reinterpret_cast<uint4*>(dst + 16 * i * a.sd[w][1]) = pack_act8<kDt>(x);
     }
   }
 }
@@ -364,8 +390,14 @@ __global__ void __launch_bounds__(256) page_copy_kernel(const __grid_constant__ 
 cudaError_t launch_page_write(const PageWriteArgs& a, cudaStream_t st) {
   // tokens of a sequence lie in at most (len + 62) / 64 + 1 pages
   const dim3 grid(unsigned((a.len + 62) / 64 + 1) * 2, a.heads, a.batch);
-  auto kern = a.fmt ? (a.dtype ? page_write_kernel<1, 1> : page_write_kernel<1, 0>)
-                    : (a.dtype ? page_write_kernel<0, 1> : page_write_kernel<0, 0>);
+  const int rope = a.rope.cos == nullptr ? 0 : (a.rope.interleaved ? 1 : 2);
+  auto pick = [&](auto fmt, auto dt) {
+    constexpr int kF = decltype(fmt)::value, kD = decltype(dt)::value;
+    return rope == 0 ? page_write_kernel<kF, kD, 0> : (rope == 1 ? page_write_kernel<kF, kD, 1> : page_write_kernel<kF, kD, 2>);
+  };
+  using Zero = std::integral_constant<int, 0>;
+  using One = std::integral_constant<int, 1>;
+  auto kern = a.fmt ? (a.dtype ? pick(One{}, One{}) : pick(One{}, Zero{})) : (a.dtype ? pick(Zero{}, One{}) : pick(Zero{}, Zero{}));
   kern<<<grid, 256, 0, st>>>(a);
   return cudaGetLastError();
 }
