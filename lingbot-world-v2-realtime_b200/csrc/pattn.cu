@@ -31,8 +31,13 @@
 
 namespace lbq {
 
-constexpr int kDecWarps = 4;
-constexpr int kDecSlots = 6;
+#ifndef DEC_SLOTS
+#define DEC_SLOTS 6
+#define DEC_CTAS 2
+#define DEC_WARPS 4
+#endif
+constexpr int kDecWarps = DEC_WARPS;
+constexpr int kDecSlots = DEC_SLOTS;
 constexpr int kMergePitch = 132;                       // floats of a merged row in shared memory
 constexpr size_t kDecSmem = 1024 + size_t(kDecSlots) * 2 * kPageBytes;
 static_assert(size_t(kDecWarps) * 16 * kMergePitch * 4 <= size_t(kDecSlots) * 2 * kPageBytes, "merge area");
@@ -116,7 +121,7 @@ struct DecShared {
 };
 
 template <int kFmt, int kDt, int kNT>
-__global__ void __launch_bounds__(kDecWarps * 32, 2)
+__global__ void __launch_bounds__(kDecWarps * 32, DEC_CTAS)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const PagedAttnArgs a) {
   constexpr int kRows = 8 * kNT;
@@ -127,13 +132,15 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
   const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles, split = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, r0 = lane >> 2;
   asm volatile("griddepcontrol.launch_dependents;");     // the merge may take its place; it waits for this grid's end
+  const int p0 = split * a.split_pages;
+  const int32_t* table = a.pt.table + b * a.pt.st_b + p0;
+  // the first page ids, before it is known whether the sequence has them: one load's latency less until data flows
+  const int id_early = threadIdx.x < kDecSlots && p0 + int(threadIdx.x) < a.pt.width ? table[threadIdx.x] : 0;
   const TileKeys tk = tile_keys(a, b, tile);
   const int pages = int((tk.visible + kPageTokens - 1) / kPageTokens);
-  const int p0 = split * a.split_pages;
   const int n = max(0, min(pages - p0, a.split_pages));
   if (split > 0 && n == 0) return;
   const bool single = pages <= a.split_pages;
-  const int32_t* table = a.pt.table + b * a.pt.st_b + p0;
   const uint32_t pool = uint32_t(a.pt.num_pages);
 
   // Page ids are loaded well before they are looked at. One outside the pool is recorded, and read as page 0 with every
@@ -168,12 +175,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
   if (threadIdx.x < kDecSlots) {
     // each slot's barrier is set up by the lane that first fills the slot
     const int s = threadIdx.x;
-    const int id = s < n ? table[s] : 0;
     mbar_init(&sh.full[s], 1);
     sh.issued[s] = 0;
     if (s == 0) sh.abort = 0;
     fence_mbar_init();
-    if (s < n) issue(s, id);
+    if (s < n) issue(s, id_early);
   }
 
   uint2 qb[kNT][8];
