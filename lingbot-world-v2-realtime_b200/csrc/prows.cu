@@ -1,27 +1,25 @@
 // Attention over the paged 8-bit KV cache, sm_100a: many query rows (prompts, whole chunks).
 //
-// The formulas of pattn.cu with both products on tcgen05. Per 128-key tile (two pages) and 128-row query tile:
+// The formulas of pattn.cu with both products on tcgen05. Per page (64 keys) and 128-row query tile:
 //   S = Q . C^T (kind::f16, fp32 in tensor memory): C the K codes widened to fp16 (exact), Q in fp16 with a power of two
 //       per row taken out; score x = S * c, c = amax_k * 2^e * softmax scale * log2 e / Q one factor a row and page
-//   P = 2^(x + log2 amax_v - m) as fp16 in tensor memory, over S; O += P . D (D the V codes in fp16)
+//   P = 2^(x + log2 amax_v - m + 7) as fp16 in tensor memory, over S; O += P . D (D the V codes in fp16)
 //   l += sum P / amax_v (fp32, before the rounding);  out = O / (Q l)
-// The scale of a V page rides in the exponent, so m is the running maximum of x + log2 amax_v: the weights that the
-// product needs are those nearest 1 and nothing overflows fp16 whatever the pages' magnitudes. m moves only when a
-// row's maximum exceeds it by more than 2^8 (weights carry a factor 2^7 and stay below 2^15), which is when O and l are
-// rescaled; the rounding of a weight is 2^-12 relative down to 2^-21 of the row's largest.
 //
-// Bound by the tensor pipe and by exp2 alike: a step (128 keys, 256 rows) has 2048 clocks of MMA (8192 flops a clock) and
-// 2048 clocks of MUFU. CTA = two 128-row query tiles of one K/V head and key split, 512 threads:
-//   warps 0-3 / 4-7  softmax of tile A / B, one thread a row (= TMEM lane): also load and scale Q, rescale O (its last
-//                    product is complete by the time the next scores are), and store the result;
-//   warps 8-11       widen the pages: global memory -> registers (one tile ahead) -> fp16 tiles in shared memory. The
+// Bound by the tensor pipe and by exp2 alike: a page and 256 rows are 1024 clocks of MMA (8192 flops a clock) and 1024
+// clocks of MUFU. CTA = two 128-row query tiles of one K/V head and key split, 512 threads:
+//   warps 0-3 / 4-7  softmax of tile A / B, one thread a row (= TMEM lane): also load and scale Q, rescale O, and store the
+//                    result;
+//   warps 8-11       widen the pages: global memory -> registers (one page ahead) -> fp16 tiles in shared memory. The
 //                    codes must pass through registers to be widened, so they are loaded there and not staged by TMA;
 //   warp 12          MMA issuer and tensor-memory owner.
-// Shared memory: Q 64 KB, K and V two fp16 stages of 32 KB each. K tiles are K-major, V tiles MN-major, and both have one
-// layout: 128-byte rows of 64 channels of a key, 128-byte swizzle, the two channel halves 16 KB apart. Tensor memory:
-// S_A, S_B, O_A, O_B, 128 columns each, P_t over the first 64 columns of S_t: the product P.D of a tile must be complete
-// before the next scores of that tile are issued (different accumulators give no order), and while it is waited for, the
-// other tile's softmax runs.
+// Shared memory: Q 64 KB, K and V four fp16 stages (pages) of 16 KB each. K tiles are K-major, V tiles MN-major, and both
+// have one layout: 128-byte rows of 64 channels of a key, 128-byte swizzle, the two channel halves 8 KB apart. Tensor
+// memory: S_A, S_B two 64-column buffers each (pages u and u + 1), O_A, O_B 128 columns, P over the first half of its S
+// buffer. The product P.D of a page must be complete before scores of page u + 2 overwrite P (different accumulators give
+// no order); meanwhile the softmax works on page u + 1. With one 128-key buffer a tile (no second page in hand) every
+// product's latency lay bare between two softmax steps: 5800 clocks for 128 keys, 1539 us for a chunk of 6032 queries x
+// 30160 keys x 12 heads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -36,23 +34,26 @@ namespace lbq {
 namespace {
 
 constexpr int kRowThreads = 512;
-constexpr int kHalf = 128 * 128;                 // bytes of 128 rows of 64 fp16 channels
-constexpr int kTile16 = 2 * kHalf;               // a 128 x 128 fp16 tile
-constexpr int kRowStages = 2;
-constexpr uint32_t kRegSoftmax = 168, kRegWiden = 128, kRegIssue = 48;
+constexpr int kQHalf = 128 * 128;                // bytes of 128 query rows of 64 fp16 channels
+constexpr int kQTile = 2 * kQHalf;
+constexpr int kHalf = 64 * 128;                  // bytes of 64 keys of 64 fp16 channels
+constexpr int kPage16 = 2 * kHalf;               // a page of fp16 values
+constexpr int kRowStages = 4;
+constexpr uint32_t kIdescScores = idesc_m128(64, 1, 0, 0);     // f32 <- f16 x f16, N = 64 keys
+constexpr uint32_t kRegSoftmax = 168, kRegWiden = 104, kRegIssue = 72;
 static_assert(128 * (2 * kRegSoftmax + kRegWiden + kRegIssue) <= kRowThreads * 128, "register split");
 struct RowsShared {
   uint64_t q_full;                               // both query tiles in shared memory (256 threads)
   uint64_t k_full[kRowStages], v_full[kRowStages];      // 128 widening threads
   uint64_t k_empty[kRowStages], v_empty[kRowStages];    // MMAs that read the stage complete
-  uint64_t s_full[2];                            // scores of tile t complete
-  uint64_t p_full[2];                            // weights of tile t written, O rescaled (128 threads)
-  uint64_t o_done[2];                            // product of tile t complete
+  uint64_t s_full[2][2];                         // [tile][page & 1]: scores complete
+  uint64_t p_full[2][2];                         // weights written, O rescaled (128 threads)
+  uint64_t o_done[2][2];                         // product complete
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
 };
-constexpr size_t kRowsSmem = 1024 + 2 * kTile16 + 2 * kRowStages * kTile16 + sizeof(RowsShared);
+constexpr size_t kRowsSmem = 1024 + 2 * kQTile + 2 * kRowStages * kPage16 + sizeof(RowsShared);
 static_assert(kRowsSmem <= 232448, "shared memory");
 
 // 16 codes -> 16 fp16 values (two 16-byte pieces).
@@ -97,25 +98,19 @@ __device__ __forceinline__ float stage_query(const uint16_t* row, uint8_t* tile,
         w[i] = pack_act2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down, 1);
       r = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *reinterpret_cast<uint4*>(tile + (c >> 3) * kHalf + rl * 128 + (((c & 7) ^ (rl & 7)) << 4)) = r;
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * kQHalf + rl * 128 + (((c & 7) ^ (rl & 7)) << 4)) = r;
   }
   return up;
 }
-
-// Page ids and scales of one 128-key tile.
-struct TileScale {
-  float ka[2], va[2];
-  bool ok[2];
-};
 
 template <int kFmt, int kDt>
 __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedAttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sK = smem + 2 * kTile16;
-  uint8_t* sV = sK + kRowStages * kTile16;
-  RowsShared* sh = reinterpret_cast<RowsShared*>(sV + kRowStages * kTile16);
+  uint8_t* sK = smem + 2 * kQTile;
+  uint8_t* sV = sK + kRowStages * kPage16;
+  RowsShared* sh = reinterpret_cast<RowsShared*>(sV + kRowStages * kPage16);
   volatile int* abort_flag = &sh->abort;
   asm volatile("griddepcontrol.launch_dependents;");     // a merge of key splits may be launched; it waits for the end
   // the last row tiles see the most keys under a causal mask: they start first
@@ -124,20 +119,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
   const TileKeys tk = tile_keys(a, b, tile);
   const int pages = int((tk.visible + kPageTokens - 1) / kPageTokens);
   const int p0 = split * a.split_pages;
-  const int np = max(0, min(pages - p0, a.split_pages));
-  if (split > 0 && np == 0) return;
-  const int n = (np + 1) / 2;                            // 128-key tiles
+  const int n = max(0, min(pages - p0, a.split_pages));
+  if (split > 0 && n == 0) return;
   const bool single = pages <= a.split_pages;
   const int32_t* table = a.pt.table + b * a.pt.st_b + p0;
-  // A page of the split, 0 with ok = false past its end or outside the pool (recorded).
-  auto page_id = [&](int i, bool& ok) {
-    ok = false;
-    if (i >= np) return 0;
-    const int id = table[i];
-    ok = id >= 0 && id < a.pt.num_pages;
-    if (!ok && a.status) atomicCAS(a.status, 0, kDevBadPage);
-    return ok ? id : 0;
-  };
+  const uint32_t pool = uint32_t(a.pt.num_pages);
 
   if (threadIdx.x == 0) {
     mbar_init(&sh->q_full, 256);
@@ -148,9 +134,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
       mbar_init(&sh->v_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&sh->s_full[t], 1);
-      mbar_init(&sh->p_full[t], 128);
-      mbar_init(&sh->o_done[t], 1);
+      for (int e = 0; e < 2; ++e) {
+        mbar_init(&sh->s_full[t][e], 1);
+        mbar_init(&sh->p_full[t][e], 128);
+        mbar_init(&sh->o_done[t][e], 1);
+      }
     }
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
@@ -169,59 +157,61 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
     reg_dealloc<kRegIssue>();
     if (warp == 12 && n > 0) {
       // ---------------------------------------------------------- MMA issuer (one lane issues)
-      const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 384};
       const uint64_t qd = smem_desc_sw128(smem_u32(sQ)), kd = smem_desc_sw128(smem_u32(sK));
       const uint64_t vd = smem_desc_sw128_mn(smem_u32(sV), kHalf);
-      constexpr uint64_t kTileDesc = kTile16 >> 4, kHalfDesc = kHalf >> 4;
-      auto scores = [&](int t, int j) {
-        const uint64_t q0 = qd + t * kTileDesc, k0 = kd + (j % kRowStages) * kTileDesc;
+      auto scores = [&](int t, int u) {
+        const uint64_t q0 = qd + t * (kQTile >> 4), k0 = kd + (u % kRowStages) * (kPage16 >> 4);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)                    // 16 channels a step, 4 steps a 64-channel half
-            mma_f16_ss(tS[t], q0 + (k >> 2) * kHalfDesc + 2 * (k & 3), k0 + (k >> 2) * kHalfDesc + 2 * (k & 3), kIdescF16,
-                       k > 0);
-          tc_commit(&sh->s_full[t]);
+            mma_f16_ss(tmem + 128 * t + 64 * (u & 1), q0 + (k >> 2) * (kQHalf >> 4) + 2 * (k & 3),
+                       k0 + (k >> 2) * (kHalf >> 4) + 2 * (k & 3), kIdescScores, k > 0);
+          tc_commit(&sh->s_full[t][u & 1]);
         }
         __syncwarp();
       };
-      bool ok = mbar_wait_role(&sh->q_full, 0, abort_flag, a.status, kDevTimeoutQ) &&
-                mbar_wait_role(&sh->k_full[0], 0, abort_flag, a.status, kDevTimeoutKV);
-      tc_fence_after();
-      if (ok) {
-        scores(0, 0);
-        scores(1, 0);
-        if (elect_one()) tc_commit(&sh->k_empty[0]);
+      auto have_k = [&](int u) {
+        return mbar_wait(&sh->k_full[u % kRowStages], (u / kRowStages) & 1, abort_flag, a.status, kDevTimeoutKV);
+      };
+      bool ok = mbar_wait_role(&sh->q_full, 0, abort_flag, a.status, kDevTimeoutQ);
+      for (int u = 0; ok && u < min(n, 2); ++u) {
+        if (!(ok = have_k(u))) break;
+        tc_fence_after();
+        scores(0, u);
+        scores(1, u);
+        if (elect_one()) tc_commit(&sh->k_empty[u]);
         __syncwarp();
       }
-      for (int j = 0; ok && j < n; ++j) {
-        const int s = j % kRowStages;
-        if (!(ok = mbar_wait(&sh->v_full[s], (j / kRowStages) & 1, abort_flag, a.status, kDevTimeoutKV))) break;
-        const bool more = j + 1 < n;
-        if (more && !(ok = mbar_wait(&sh->k_full[(j + 1) % kRowStages], ((j + 1) / kRowStages) & 1, abort_flag, a.status,
-                                     kDevTimeoutKV)))
-          break;
+      for (int u = 0; ok && u < n; ++u) {
+        const int s = u % kRowStages, e = u & 1;
+        const uint32_t phase = (u >> 1) & 1;
+        if (!(ok = mbar_wait(&sh->v_full[s], (u / kRowStages) & 1, abort_flag, a.status, kDevTimeoutKV))) break;
         for (int t = 0; ok && t < 2; ++t) {
-          if (!(ok = mbar_wait(&sh->p_full[t], j & 1, abort_flag, a.status, kDevTimeoutP))) break;
+          if (!(ok = mbar_wait(&sh->p_full[t][e], phase, abort_flag, a.status, kDevTimeoutP))) break;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)                  // 16 keys a step: 8 columns of P, 2 groups of 8 rows of V
-              mma_f16_ts(tO[t], tS[t] + 8 * k, vd + s * kTileDesc + k * (2048 >> 4), kIdescF16BMn, j > 0 || k > 0);
-            tc_commit(&sh->o_done[t]);
+            for (int k = 0; k < 4; ++k)                  // 16 keys a step: 8 columns of P, 2 groups of 8 rows of V
+              mma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 64 * e + 8 * k, vd + s * (kPage16 >> 4) + k * (2048 >> 4),
+                         kIdescF16BMn, u > 0 || k > 0);
+            tc_commit(&sh->o_done[t][e]);
           }
           __syncwarp();
-          if (more) {
-            if (!(ok = mbar_wait(&sh->o_done[t], j & 1, abort_flag, a.status, kDevTimeoutO))) break;
-            tc_fence_after();
-            scores(t, j + 1);
-          }
         }
         if (!ok) break;
-        if (elect_one()) {
-          tc_commit(&sh->v_empty[s]);
-          if (more) tc_commit(&sh->k_empty[(j + 1) % kRowStages]);
-        }
+        if (elect_one()) tc_commit(&sh->v_empty[s]);
         __syncwarp();
+        if (u + 2 < n) {
+          if (!(ok = have_k(u + 2))) break;
+          for (int t = 0; ok && t < 2; ++t) {
+            if (!(ok = mbar_wait(&sh->o_done[t][e], phase, abort_flag, a.status, kDevTimeoutO))) break;
+            tc_fence_after();
+            scores(t, u + 2);
+          }
+          if (!ok) break;
+          if (elect_one()) tc_commit(&sh->k_empty[(u + 2) % kRowStages]);
+          __syncwarp();
+        }
       }
       if (elect_one()) tc_commit(&sh->drain);            // every MMA has completed once it flips
       __syncwarp();
@@ -231,162 +221,155 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
     // ------------------------------------------------------------ widening warps
     reg_dealloc<kRegWiden>();
     const int w = warp - 8, kr = lane & 7, c4 = lane >> 3;
-    // piece i of a tile: key 8 * (u / 2) + kr, 16-byte piece 4 * (u % 2) + c4 of its row, u = 4 i + w. Eight lanes of a
+    // piece i of a page: key 8 * (q / 2) + kr, 16-byte piece 4 * (q % 2) + c4 of its row, q = 4 i + w. Eight lanes of a
     // store take eight keys, whose swizzle spreads them over all banks.
-    auto load = [&](const uint8_t* base, int j, uint4 (&r)[8]) {
-      bool ok[2];
-      const uint8_t* pg[2];
+    auto load = [&](const uint8_t* base, int u, int id, uint4 (&r)[4]) {
+      const bool ok = uint32_t(id) < pool;
+      if (!ok && a.status) atomicCAS(a.status, 0, kDevBadPage);
+      const uint8_t* pg = base + (int64_t(ok ? id : 0) * a.heads + h) * kPageBytes;
+      // rows past the sequence hold what the page held before: a NaN code times a weight of 0 would be NaN
+      const int64_t rest = ok ? tk.kv - int64_t(p0 + u) * kPageTokens : 0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int64_t id = page_id(2 * j + e, ok[e]);
-        pg[e] = base + (id * a.heads + h) * kPageBytes;
-      }
-      const int64_t k0 = int64_t(p0 + 2 * j) * kPageTokens;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int u = 4 * i + w, key = (u >> 1) * 8 + kr;
-        // rows past the sequence hold what the page held before: a NaN code times a weight of 0 would be NaN
-        r[i] = ok[i >> 2] && k0 + key < tk.kv
-                   ? *reinterpret_cast<const uint4*>(pg[i >> 2] + (key & 63) * 128 + ((u & 1) * 4 + c4) * 16)
-                   : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < 4; ++i) {
+        const int q = 4 * i + w, key = (q >> 1) * 8 + kr;
+        r[i] = key < rest ? *reinterpret_cast<const uint4*>(pg + key * 128 + ((q & 1) * 4 + c4) * 16) : make_uint4(0u, 0u, 0u, 0u);
       }
     };
-    auto store = [&](uint8_t* dst, const uint4 (&r)[8]) {
+    auto store = [&](uint8_t* dst, const uint4 (&r)[4]) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int u = 4 * i + w, key = (u >> 1) * 8 + kr;
+      for (int i = 0; i < 4; ++i) {
+        const int q = 4 * i + w, key = (q >> 1) * 8 + kr;
         uint4 lo, hi;
         widen16<kFmt>(r[i], lo, hi);
-        uint8_t* row = dst + (u & 1) * kHalf + key * 128;
+        uint8_t* row = dst + (q & 1) * kHalf + key * 128;
         *reinterpret_cast<uint4*>(row + (((2 * c4) ^ kr) << 4)) = lo;
         *reinterpret_cast<uint4*>(row + (((2 * c4 + 1) ^ kr) << 4)) = hi;
       }
       fence_proxy_async_smem();
     };
-    uint4 kreg[8], vreg[8];
+    uint4 kreg[4], vreg[4];
+    int id_next = 0;
     if (n > 0) {
-      load(a.k_pages, 0, kreg);
-      load(a.v_pages, 0, vreg);
+      const int id = table[0];
+      load(a.k_pages, 0, id, kreg);
+      load(a.v_pages, 0, id, vreg);
+      if (n > 1) id_next = table[1];
     }
-    for (int j = 0; j < n; ++j) {
-      const int s = j % kRowStages;
-      const uint32_t phase = ((j / kRowStages) & 1) ^ 1;
+    for (int u = 0; u < n; ++u) {
+      const int s = u % kRowStages;
+      const uint32_t phase = ((u / kRowStages) & 1) ^ 1;
+      const int id = id_next;
+      if (u + 2 < n) id_next = table[u + 2];
       if (!mbar_wait_role(&sh->k_empty[s], phase, abort_flag, a.status, kDevTimeoutKV)) break;
-      store(sK + s * kTile16, kreg);
+      store(sK + s * kPage16, kreg);
       mbar_arrive(&sh->k_full[s]);
-      if (j + 1 < n) load(a.k_pages, j + 1, kreg);
+      if (u + 1 < n) load(a.k_pages, u + 1, id, kreg);
       if (!mbar_wait_role(&sh->v_empty[s], phase, abort_flag, a.status, kDevTimeoutKV)) break;
-      store(sV + s * kTile16, vreg);
+      store(sV + s * kPage16, vreg);
       mbar_arrive(&sh->v_full[s]);
-      if (j + 1 < n) load(a.v_pages, j + 1, vreg);
+      if (u + 1 < n) load(a.v_pages, u + 1, id, vreg);
     }
   } else {
     // ------------------------------------------------------------ softmax warps
     reg_alloc<kRegSoftmax>();
     const int t = warp >> 2, quarter = warp & 3, rl = quarter * 32 + lane;
     const uint32_t lane_off = uint32_t(quarter * 32) << 16;
-    const uint32_t tS = tmem + 128 * t + lane_off, tO = tmem + 256 + 128 * t + lane_off;
+    const uint32_t tS0 = tmem + 128 * t + lane_off, tO = tmem + 256 + 128 * t + lane_off;
     const int row = tile * kManyTile + t * 128 + rl, qi = row / a.group, head = h * a.group + (row - qi * a.group);
     const bool on = qi < tk.qn;
     const uint16_t* qrow = on ? static_cast<const uint16_t*>(a.q) + b * a.sq[0] + qi * a.sq[1] + head * a.sq[2] : nullptr;
-    const float unit = stage_query<kDt>(qrow, sQ + t * kTile16, rl) * a.score_log2;
+    const float unit = stage_query<kDt>(qrow, sQ + t * kQTile, rl) * a.score_log2;
     fence_proxy_async_smem();
     mbar_arrive(&sh->q_full);
     const int64_t limit = (!on ? -1 : (a.causal ? tk.kv - tk.qn + qi : tk.kv - 1)) - int64_t(p0) * kPageTokens;
     float m = -INFINITY, l = 0.f;
-    auto scales = [&](int j) {
-      TileScale x;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int64_t id = page_id(2 * j + e, x.ok[e]);
-        // kept above 0 (a written page's are at least 2^-40): a masked score is -inf times ka, and va is divided by
-        x.ka[e] = x.ok[e] ? fmaxf(a.ka[id * a.heads + h], kTinyScale) : 1.f;
-        x.va[e] = x.ok[e] ? fmaxf(a.va[id * a.heads + h], kTinyScale) : 1.f;
-      }
-      return x;
+    // The scales of the next page are loaded one page ahead, its id two pages ahead. They are kept above 0 (a written
+    // page's are at least 2^-40): a masked score is -inf times ka, and va is divided by.
+    int id_next = n > 0 ? table[0] : 0;
+    float ka_next = 1.f, va_next = 1.f;
+    bool ok_next = false;
+    auto scales = [&](int u) {
+      ok_next = uint32_t(id_next) < pool;
+      const int64_t at = int64_t(ok_next ? id_next : 0) * a.heads + h;
+      ka_next = a.ka[at];
+      va_next = a.va[at];
+      if (u + 1 < n) id_next = table[u + 1];
     };
-    TileScale next{};
-    if (n > 0) next = scales(0);
+    if (n > 0) scales(0);
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      const TileScale sc = next;
-      if (j + 1 < n) next = scales(j + 1);
-      if (!(ok = mbar_wait(&sh->s_full[t], j & 1, abort_flag, a.status, kDevTimeoutS))) break;
+    for (int u = 0; u < n; ++u) {
+      const bool known = ok_next;
+      const float ka = fmaxf(ka_next, kTinyScale), va = fmaxf(va_next, kTinyScale);
+      if (u + 1 < n) scales(u + 1);
+      const uint32_t tS = tS0 + 64 * (u & 1);
+      if (!(ok = mbar_wait(&sh->s_full[t][u & 1], (u >> 1) & 1, abort_flag, a.status, kDevTimeoutS))) break;
       tc_fence_after();
-      uint32_t sv[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sv[32 * c]));
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        auto& part = *reinterpret_cast<uint32_t(*)[32]>(&sv[32 * c]);
-        if (c == 0) tmem_ld_wait(part);
-        else reg_anchor(part);
-      }
+      uint32_t sv[64];
+      auto& sv0 = *reinterpret_cast<uint32_t(*)[32]>(&sv[0]);
+      auto& sv1 = *reinterpret_cast<uint32_t(*)[32]>(&sv[32]);
+      tmem_ld32(tS, sv0);
+      tmem_ld32(tS + 32, sv1);
+      tmem_ld_wait(sv0);
+      reg_anchor(sv1);
       auto F = [&](int i) { return __uint_as_float(sv[i]); };
-      const int64_t rest = limit - int64_t(j) * 128;      // last visible key of the tile
-      if (!__all_sync(0xffffffffu, rest >= 127 && sc.ok[0] && sc.ok[1])) {
-        const int last0 = sc.ok[0] ? int(rest < 64 ? rest : 63) : -1, last1 = sc.ok[1] ? int(rest < 128 ? rest : 127) : -1;
+      const int64_t rest = limit - int64_t(u) * kPageTokens;   // last visible key of the page
+      if (!__all_sync(0xffffffffu, rest >= 63 && known)) {
+        const int last = known ? int(rest < 63 ? (rest < 0 ? -1 : rest) : 63) : -1;
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i > (i < 64 ? last0 : last1)) sv[i] = 0xff800000u;
+        for (int i = 0; i < 64; ++i)
+          if (i > last) sv[i] = 0xff800000u;
       }
-      float r[8];
+      float r[4];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) r[q] = fmaxf(F(64 * (q >> 2) + 2 * (q & 3)), F(64 * (q >> 2) + 2 * (q & 3) + 1));
+      for (int q = 0; q < 4; ++q) r[q] = fmaxf(F(2 * q), F(2 * q + 1));
 #pragma unroll
       for (int i = 8; i < 64; i += 8) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          r[q] = fmax3(r[q], F(i + 2 * q), F(i + 2 * q + 1));
-          r[4 + q] = fmax3(r[4 + q], F(64 + i + 2 * q), F(64 + i + 2 * q + 1));
-        }
+        for (int q = 0; q < 4; ++q) r[q] = fmax3(r[q], F(i + 2 * q), F(i + 2 * q + 1));
       }
-      const float c0 = sc.ka[0] * unit, c1 = sc.ka[1] * unit;
-      const float lv0 = __log2f(sc.va[0]), lv1 = __log2f(sc.va[1]);
-      const float x0 = fmax3(r[0], r[1], fmaxf(r[2], r[3])), x1 = fmax3(r[4], r[5], fmaxf(r[6], r[7]));
-      const float top = fmaxf(fmaf(x0, c0, lv0), fmaf(x1, c1, lv1));
+      const float c = ka * unit, lv = __log2f(va);
+      const float top = fmaf(fmax3(r[0], r[1], fmaxf(r[2], r[3])), c, lv);
       const bool grow = top > m + kSlack;                 // also from m = -inf
       if (__any_sync(0xffffffffu, grow)) {
         const float alpha = grow ? ex2_approx(m - top) : 1.f;
         if (grow) m = top;
         l *= alpha;
-        if (j > 0) {
+        if (u > 0) {                                      // products up to page u - 2 are complete, as its scores are
+          if (!(ok = mbar_wait(&sh->o_done[t][(u - 1) & 1], ((u - 1) >> 1) & 1, abort_flag, a.status, kDevTimeoutO))) break;
+          tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
+          for (int cc = 0; cc < 4; ++cc) {
             uint32_t ov[32];
-            tmem_ld32(tO + 32 * c, ov);
+            tmem_ld32(tO + 32 * cc, ov);
             tmem_ld_wait(ov);
 #pragma unroll
             for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-            tmem_st32(tO + 32 * c, ov);
+            tmem_st32(tO + 32 * cc, ov);
           }
         }
       }
-      const float ref = (m == -INFINITY ? 0.f : m) - kWeightBits;
-      const uint64_t cc[2] = {f2_pack(c0, c0), f2_pack(c1, c1)};
-      const uint64_t bb[2] = {f2_pack(lv0 - ref, lv0 - ref), f2_pack(lv1 - ref, lv1 - ref)};
-      uint64_t acc[4] = {0, 0, 0, 0};
+      const float ref = lv - ((m == -INFINITY ? 0.f : m) - kWeightBits);
+      const uint64_t c2 = f2_pack(c, c), b2 = f2_pack(ref, ref);
+      uint64_t acc[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        const int e = i >> 5;
+      for (int i = 0; i < 32; ++i) {
         float w0, w1;
-        f2_unpack(f2_fma(f2_pack(F(2 * i), F(2 * i + 1)), cc[e], bb[e]), w0, w1);
+        f2_unpack(f2_fma(f2_pack(F(2 * i), F(2 * i + 1)), c2, b2), w0, w1);
         w0 = ex2_approx(w0);
         w1 = ex2_approx(w1);
-        acc[2 * e + (i & 1)] = f2_add(acc[2 * e + (i & 1)], f2_pack(w0, w1));
+        acc[i & 1] = f2_add(acc[i & 1], f2_pack(w0, w1));
         sv[i] = pack_act2(w0, w1, 1);
       }
-      tmem_st32(tS, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
-      tmem_st32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+      tmem_st32(tS, sv0);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&sh->p_full[t]);
-      float s[8];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) f2_unpack(acc[q], s[2 * q], s[2 * q + 1]);
-      l += __fdividef((s[0] + s[1]) + (s[2] + s[3]), sc.va[0]) + __fdividef((s[4] + s[5]) + (s[6] + s[7]), sc.va[1]);
+      mbar_arrive(&sh->p_full[t][u & 1]);
+      float s[4];
+      f2_unpack(acc[0], s[0], s[1]);
+      f2_unpack(acc[1], s[2], s[3]);
+      l += __fdividef((s[0] + s[1]) + (s[2] + s[3]), va);
     }
-    if (ok && n > 0) ok = mbar_wait(&sh->o_done[t], (n - 1) & 1, abort_flag, a.status, kDevTimeoutO);
+    if (ok && n > 0) ok = mbar_wait(&sh->o_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, a.status, kDevTimeoutO);
     tc_fence_after();
     // ---------------------------------------------------------- result: O / (Q l), or the split's O / Q, m - 7, l
     const bool row_ok = ok && qi < a.q_len;
