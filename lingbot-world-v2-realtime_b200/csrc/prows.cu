@@ -56,12 +56,11 @@ struct RowsShared {
 constexpr size_t kRowsSmem = 1024 + 2 * kQTile + 2 * kRowStages * kPage16 + sizeof(RowsShared);
 static_assert(kRowsSmem <= 232448, "shared memory");
 
-// 16 codes -> 16 fp16 values (two 16-byte pieces).
+// 8 codes -> 8 fp16 values.
 template <int kFmt>
-__device__ __forceinline__ void widen16(const uint4 r, uint4& lo, uint4& hi) {
-  const uint32_t w[4] = {bias<kFmt>(r.x), bias<kFmt>(r.y), bias<kFmt>(r.z), bias<kFmt>(r.w)};
-  lo = make_uint4(widen<kFmt, 0, 1>(w[0]), widen<kFmt, 2, 3>(w[0]), widen<kFmt, 0, 1>(w[1]), widen<kFmt, 2, 3>(w[1]));
-  hi = make_uint4(widen<kFmt, 0, 1>(w[2]), widen<kFmt, 2, 3>(w[2]), widen<kFmt, 0, 1>(w[3]), widen<kFmt, 2, 3>(w[3]));
+__device__ __forceinline__ uint4 widen8(const uint2 r) {
+  const uint32_t a = bias<kFmt>(r.x), b = bias<kFmt>(r.y);
+  return make_uint4(widen<kFmt, 0, 1>(a), widen<kFmt, 2, 3>(a), widen<kFmt, 0, 1>(b), widen<kFmt, 2, 3>(b));
 }
 
 // One query row (null: zeros) as fp16 into row rl of a swizzled tile, scaled by a power of two to a maximum in [1, 2)
@@ -220,9 +219,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
   } else if (warp >= 8) {
     // ------------------------------------------------------------ widening warps
     reg_dealloc<kRegWiden>();
-    const int w = warp - 8, kr = lane & 7, c4 = lane >> 3;
-    // piece i of a page: key 8 * (q / 2) + kr, 16-byte piece 4 * (q % 2) + c4 of its row, q = 4 i + w. Eight lanes of a
-    // store take eight keys, whose swizzle spreads them over all banks.
+    const int w = warp - 8, c = lane & 7, half = c >> 2;
+    // piece i of a page: key 16 i + 4 w + lane / 8, 16-byte piece c of its row: a load takes four whole 128-byte rows.
+    // Its 16 values are two 16-byte pieces of the key's row in channel half `half`; the lanes of one half store the first
+    // one first and those of the other the second, so that the eight lanes of a key take all eight bank groups at once.
     auto load = [&](const uint8_t* base, int u, int id, uint4 (&r)[4]) {
       const bool ok = uint32_t(id) < pool;
       if (!ok && a.status) atomicCAS(a.status, 0, kDevBadPage);
@@ -231,19 +231,19 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
       const int64_t rest = ok ? tk.kv - int64_t(p0 + u) * kPageTokens : 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int q = 4 * i + w, key = (q >> 1) * 8 + kr;
-        r[i] = key < rest ? *reinterpret_cast<const uint4*>(pg + key * 128 + ((q & 1) * 4 + c4) * 16) : make_uint4(0u, 0u, 0u, 0u);
+        const int key = 16 * i + 4 * w + (lane >> 3);
+        r[i] = key < rest ? *reinterpret_cast<const uint4*>(pg + key * 128 + c * 16) : make_uint4(0u, 0u, 0u, 0u);
       }
     };
     auto store = [&](uint8_t* dst, const uint4 (&r)[4]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int q = 4 * i + w, key = (q >> 1) * 8 + kr;
-        uint4 lo, hi;
-        widen16<kFmt>(r[i], lo, hi);
-        uint8_t* row = dst + (q & 1) * kHalf + key * 128;
-        *reinterpret_cast<uint4*>(row + (((2 * c4) ^ kr) << 4)) = lo;
-        *reinterpret_cast<uint4*>(row + (((2 * c4 + 1) ^ kr) << 4)) = hi;
+        const int key = 16 * i + 4 * w + (lane >> 3), k7 = key & 7, at = 2 * (c & 3);
+        uint8_t* row = dst + half * kHalf + key * 128;
+        const uint2 first = half ? make_uint2(r[i].z, r[i].w) : make_uint2(r[i].x, r[i].y);
+        const uint2 second = half ? make_uint2(r[i].x, r[i].y) : make_uint2(r[i].z, r[i].w);
+        *reinterpret_cast<uint4*>(row + (((at + half) ^ k7) << 4)) = widen8<kFmt>(first);
+        *reinterpret_cast<uint4*>(row + (((at + 1 - half) ^ k7) << 4)) = widen8<kFmt>(second);
       }
       fence_proxy_async_smem();
     };
