@@ -8,6 +8,16 @@
 
 namespace lbq {
 
+// Start of every kernel of this family: nothing is read or written before the grid that it follows in its stream has
+// ended; then the next launch may take its place on the GPU as SMs allow. They are launched with programmatic stream
+// serialization (launch_after below), so the launch latency and the set-up of one overlap the run of the one before. Every
+// thread comes through here, so that a grid never ends before the grids it follows, and when a grid starts all but the one
+// directly before it have ended.
+__device__ __forceinline__ void after_previous_grid() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 constexpr float kTinyScale = 5.421010862427522e-20f;   // 2^-64: scales are kept above it (a written page's are >= 2^-40)
 constexpr float kWeightBits = 7.f;               // weights are scaled by 2^7 ...
 constexpr float kSlack = 8.f;                    // ... and the running maximum may lag by 2^8: below 2^15, fp16's range
@@ -54,6 +64,21 @@ __device__ __forceinline__ uint32_t bias(uint32_t r) { return kFmt == 0 ? r ^ 0x
 
 __device__ __forceinline__ float natural_lse(float m, float l) {
   return l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : (l == l ? -INFINITY : l);
+}
+
+template <class... Params, class... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
 }
 
 }  // namespace lbq

@@ -20,6 +20,7 @@
 
 #include "lbq_kernels.h"
 #include "lbq_paged.h"
+#include "lbq_paged.cuh"
 #include "lbq_ptx.cuh"
 
 namespace lbq {
@@ -305,6 +306,7 @@ __device__ __forceinline__ void write_page(const PageWriteArgs& a, const int w, 
 template <int kFmt, int kDt, int kRope>
 __global__ void __launch_bounds__(256) page_write_kernel(const __grid_constant__ PageWriteArgs a) {
   __shared__ uint32_t red[8];
+  after_previous_grid();
   if (blockIdx.x & 1) write_page<kFmt, kDt, 0>(a, 1, red);
   else write_page<kFmt, kDt, kRope>(a, 0, red);
 }
@@ -316,6 +318,7 @@ template <int kFmt, int kDt>
 __global__ void __launch_bounds__(256) page_read_kernel(const __grid_constant__ PageReadArgs a) {
   const int h = blockIdx.y, b = blockIdx.z;
   const int t = threadIdx.x, c16 = t & 15, rg = t >> 4;
+  after_previous_grid();
   const int64_t start = a.start ? a.start[b] : a.start0;
   int n = a.lens ? a.lens[b] : a.len;
   n = n < 0 ? 0 : (n > a.len ? a.len : n);
@@ -363,6 +366,7 @@ __global__ void __launch_bounds__(256) page_read_kernel(const __grid_constant__ 
 // tensor); the pair list travels in the parameters, so nothing is read before the data.
 __global__ void __launch_bounds__(256) page_copy_kernel(const __grid_constant__ PageCopyArgs a) {
   const int w = blockIdx.z & 1, layer = blockIdx.z >> 1;
+  after_previous_grid();
   const int64_t page = int64_t(a.heads) * kPageBytes;
   const int64_t src = a.src[blockIdx.y], dst = a.dst[blockIdx.y];
   uint8_t* base = a.codes[w] + layer * a.layer_codes;
@@ -398,20 +402,17 @@ cudaError_t launch_page_write(const PageWriteArgs& a, cudaStream_t st) {
   using Zero = std::integral_constant<int, 0>;
   using One = std::integral_constant<int, 1>;
   auto kern = a.fmt ? (a.dtype ? pick(One{}, One{}) : pick(One{}, Zero{})) : (a.dtype ? pick(Zero{}, One{}) : pick(Zero{}, Zero{}));
-  kern<<<grid, 256, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_after(kern, grid, dim3(256), 0, st, a);
 }
 cudaError_t launch_page_read(const PageReadArgs& a, cudaStream_t st) {
   const dim3 grid(unsigned((a.len + 63) / 64), a.heads, a.batch);
   auto kern = a.fmt ? (a.dtype ? page_read_kernel<1, 1> : page_read_kernel<1, 0>)
                     : (a.dtype ? page_read_kernel<0, 1> : page_read_kernel<0, 0>);
-  kern<<<grid, 256, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_after(kern, grid, dim3(256), 0, st, a);
 }
 cudaError_t launch_page_copy(const PageCopyArgs& a, cudaStream_t st) {
   const dim3 grid(unsigned((int64_t(a.heads) * kPageBytes / 16 + 1023) / 1024), a.pairs, a.layers * 2);
-  page_copy_kernel<<<grid, 256, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_after(page_copy_kernel, grid, dim3(256), 0, st, a);
 }
 
 }  // namespace lbq

@@ -31,13 +31,8 @@
 
 namespace lbq {
 
-#ifndef DEC_SLOTS
-#define DEC_SLOTS 6
-#define DEC_CTAS 2
-#define DEC_WARPS 4
-#endif
-constexpr int kDecWarps = DEC_WARPS;
-constexpr int kDecSlots = DEC_SLOTS;
+constexpr int kDecWarps = 4;
+constexpr int kDecSlots = 6;
 constexpr int kMergePitch = 132;                       // floats of a merged row in shared memory
 constexpr size_t kDecSmem = 1024 + size_t(kDecSlots) * 2 * kPageBytes;
 static_assert(size_t(kDecWarps) * 16 * kMergePitch * 4 <= size_t(kDecSlots) * 2 * kPageBytes, "merge area");
@@ -121,7 +116,7 @@ struct DecShared {
 };
 
 template <int kFmt, int kDt, int kNT>
-__global__ void __launch_bounds__(kDecWarps * 32, DEC_CTAS)
+__global__ void __launch_bounds__(kDecWarps * 32, 2)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const PagedAttnArgs a) {
   constexpr int kRows = 8 * kNT;
@@ -131,7 +126,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, DEC_CTAS)
   volatile int* abort_flag = &sh.abort;
   const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles, split = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, r0 = lane >> 2;
-  asm volatile("griddepcontrol.launch_dependents;");     // the merge may take its place; it waits for this grid's end
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  after_previous_grid();
   const int p0 = split * a.split_pages;
   const int32_t* table = a.pt.table + b * a.pt.st_b + p0;
   // the first page ids, before it is known whether the sequence has them: one load's latency less until data flows
@@ -432,14 +431,14 @@ __global__ void __launch_bounds__(kDecWarps * 32, DEC_CTAS)
 
 // Merge of the key splits: one CTA a row, its 4 warps take the splits in turn, 4 channels a lane. A split's weight is
 // 2^(m_s - max m). Rows whose tile fits one split were finished by the attention kernel. Few rows with many splits are
-// the common case (a decoded token): what counts is latency, so the splits' loads do not wait for one another, and the
-// launch overlaps the attention kernel's (programmatic dependent launch).
+// the common case (a decoded token): what counts is latency, so up to 32 splits' loads go out together.
 template <int kDt>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs a) {
   const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // the lengths are the caller's, written before the attention kernel, which let this grid start only after it had waited
   const TileKeys tk = tile_keys(a, b, row / a.tile_rows);
+  after_previous_grid();
   const int pages = int((tk.visible + kPageTokens - 1) / kPageTokens);
   if (pages <= a.split_pages) return;
   const int n = (pages + a.split_pages - 1) / a.split_pages;
@@ -449,11 +448,12 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs 
   __shared__ float4 so[4][32];
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = warp; s0 < n; s0 += 16) {                  // four splits a round
-    float2 ml[4];
-    float4 x[4];
+  constexpr int kRound = 8;                                // splits a warp loads at once
+  for (int s0 = warp; s0 < n; s0 += 4 * kRound) {
+    float2 ml[kRound];
+    float4 x[kRound];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kRound; ++k) {
       const int s = s0 + 4 * k;
       ml[k] = make_float2(-INFINITY, 0.f);
       x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -462,13 +462,15 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs 
         x[k] = *reinterpret_cast<const float4*>(a.o_part + (s * step + at) * 128 + 4 * lane);
       }
     }
-    const float top = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < kRound; ++k) top = fmaxf(top, ml[k].x);
     const float ref = top == -INFINITY ? 0.f : top, al = ex2_approx(m - ref);
     m = top;
     l *= al;
     o = make_float4(o.x * al, o.y * al, o.z * al, o.w * al);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kRound; ++k) {
       const float f = ex2_approx(ml[k].x - ref);
       l += ml[k].y * f;
       o.x += x[k].x * f;
@@ -510,8 +512,7 @@ template <int kFmt, int kDt, int kNT>
 cudaError_t launch_decode_as(const PagedAttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
   if (cudaError_t e = allow_dynamic_smem<paged_decode_kernel<kFmt, kDt, kNT>>(int(kDecSmem)); e != cudaSuccess) return e;
   const dim3 grid(unsigned(a.heads) * a.tiles, a.splits, a.batch);
-  paged_decode_kernel<kFmt, kDt, kNT><<<grid, kDecWarps * 32, kDecSmem, st>>>(tm_k, tm_v, a);
-  return cudaGetLastError();
+  return launch_after(paged_decode_kernel<kFmt, kDt, kNT>, grid, dim3(kDecWarps * 32), kDecSmem, st, tm_k, tm_v, a);
 }
 template <int kFmt, int kDt>
 cudaError_t launch_decode_rows(const PagedAttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
@@ -523,16 +524,9 @@ cudaError_t launch_paged_decode(const PagedAttnArgs& a, const CUtensorMap& tm_k,
   return a.dtype ? launch_decode_rows<0, 1>(a, tm_k, tm_v, st) : launch_decode_rows<0, 0>(a, tm_k, tm_v, st);
 }
 cudaError_t launch_paged_combine(const PagedAttnArgs& a, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(a.q_len) * a.group, a.heads, a.batch);
-  cfg.blockDim = dim3(128);
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return a.dtype ? cudaLaunchKernelEx(&cfg, paged_combine_kernel<1>, a) : cudaLaunchKernelEx(&cfg, paged_combine_kernel<0>, a);
+  const dim3 grid(unsigned(a.q_len) * a.group, a.heads, a.batch);
+  return a.dtype ? launch_after(paged_combine_kernel<1>, grid, dim3(128), 0, st, a)
+                 : launch_after(paged_combine_kernel<0>, grid, dim3(128), 0, st, a);
 }
 
 }  // namespace lbq

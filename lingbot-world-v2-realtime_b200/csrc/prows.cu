@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
   uint8_t* sV = sK + kRowStages * kPage16;
   RowsShared* sh = reinterpret_cast<RowsShared*>(sV + kRowStages * kPage16);
   volatile int* abort_flag = &sh->abort;
-  asm volatile("griddepcontrol.launch_dependents;");     // a merge of key splits may be launched; it waits for the end
+  after_previous_grid();
   // the last row tiles see the most keys under a causal mask: they start first
   const int tile = a.tiles - 1 - int(blockIdx.x % a.tiles), h = blockIdx.x / a.tiles, split = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -423,8 +423,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
 template <int kFmt, int kDt>
 cudaError_t launch_rows_as(const PagedAttnArgs& a, cudaStream_t st) {
   if (cudaError_t e = allow_dynamic_smem<paged_rows_kernel<kFmt, kDt>>(int(kRowsSmem)); e != cudaSuccess) return e;
-  paged_rows_kernel<kFmt, kDt><<<dim3(unsigned(a.heads) * a.tiles, a.splits, a.batch), kRowThreads, kRowsSmem, st>>>(a);
-  return cudaGetLastError();
+  return launch_after(paged_rows_kernel<kFmt, kDt>, dim3(unsigned(a.heads) * a.tiles, a.splits, a.batch), dim3(kRowThreads),
+                      kRowsSmem, st, a);
 }
 
 }  // namespace

@@ -13,6 +13,7 @@
 
 #include "lbq_kernels.h"
 #include "lbq_paged.h"
+#include "lbq_paged.cuh"
 #include "lbq_ptx.cuh"
 
 namespace lbq {
@@ -104,7 +105,7 @@ struct Piece {
 // every blockDim.y-th head of each tensor, two at a time: the loads of two heads of both tensors go out before the table
 // row is there, and the addresses advance by one addition a head.
 template <int kDt, bool kInter, int kN>
-__global__ void __launch_bounds__(512) rope_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeArgs a) {
   using T = typename ActType<kDt>::T;
   constexpr int kPairs = kInter ? kN / 2 : kN;
   const int u = threadIdx.x, l = blockIdx.x, b = blockIdx.y;
@@ -112,6 +113,7 @@ __global__ void __launch_bounds__(512) rope_kernel(const RopeArgs a) {
   const int rot_units = kInter ? a.rope.rot / kN : half / kN;
   const bool turn = u < rot_units;
   const int ch = turn ? u * kN : a.rope.rot + (u - rot_units) * kN;
+  after_previous_grid();
   int64_t row = a.start + l;
   if (a.rope.pos != nullptr) {
     const int64_t at = b * a.rope.sp_b + l * a.rope.sp_l;
@@ -206,8 +208,7 @@ cudaError_t launch_rope_as(const RopeArgs& a, cudaStream_t st) {
   int hy = int64_t(a.batch) * a.len >= 1024 ? (most + 1) / 2 : most;
   const int fit = units >= 512 ? 1 : 512 / units;
   if (hy > fit) hy = fit;
-  rope_kernel<kDt, kInter, kN><<<dim3(a.len, a.batch), dim3(units, hy), 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_after(rope_kernel<kDt, kInter, kN>, dim3(a.len, a.batch), dim3(units, hy), 0, st, a);
 }
 template <int kDt>
 cudaError_t launch_rope_dt(const RopeArgs& a, cudaStream_t st) {
