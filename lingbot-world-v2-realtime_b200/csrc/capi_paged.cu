@@ -262,10 +262,15 @@ int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t ma
   const int tile = attn_tile_rows(rows);
   const int64_t ctas = (rows + tile - 1) / tile * heads * batch;
   const int64_t pages = (max_kv_len + lbq::kPageTokens - 1) / lbq::kPageTokens;
-  // few rows: two CTAs an SM, a split keeps at least 4 pages, one for each warp; many rows: one CTA an SM, at least
-  // 8 pages (4 key tiles) to pay for the query tiles
-  int64_t n = (tile != lbq::kManyTile ? 2 * 148 : 148) / ctas;
-  const int64_t least = tile != lbq::kManyTile ? 4 : 8;
+  // Few rows: two CTAs an SM (296 at once), a split keeps at least 4 pages, one for each warp. From 90 CTAs on, where
+  // rounding down would leave a third of them idle, one more; up to 400, where one split each would nearly fill the GPU, two
+  // for long windows all the same, since sequences of a batch are seldom alike (measured, us, 1 / 2 / 4 splits of 256 CTAs of
+  // 8192 keys: all alike 84 / 93 / 100, lengths spread 1..8192 79 / 65 / 61; 3 / 4 / 6 of 96 ragged CTAs 25 / 22 / 19).
+  // Many rows: one CTA an SM, at least 8 pages to pay for the query tiles.
+  const bool few = tile != lbq::kManyTile;
+  int64_t n = (few ? 2 * 148 : 148) / ctas;
+  if (few && ctas >= 90 && ctas <= 400 && pages >= 32) n = ctas <= 148 ? n + 1 : 2;
+  const int64_t least = few ? 4 : 8;
   if (n > pages / least) n = pages / least;
   return int(n < 1 ? 1 : (n > 1024 ? 1024 : n));
 }

@@ -15,6 +15,7 @@
 
 #include <Python.h>
 #include <cstdint>
+#include <vector>
 
 #include "../../include/lbq.h"
 
@@ -24,17 +25,18 @@ namespace {
 decltype(&lbq_rope) f_rope = nullptr;
 decltype(&lbq_page_write) f_write = nullptr;
 decltype(&lbq_page_read) f_read = nullptr;
+decltype(&lbq_page_copy) f_copy = nullptr;
 decltype(&lbq_paged_attn) f_attn = nullptr;
 decltype(&lbq_paged_attn_splits) f_splits = nullptr;
 decltype(&lbq_paged_attn_workspace) f_workspace = nullptr;
 
 PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 6) {
-    PyErr_SetString(PyExc_TypeError, "init takes the addresses of 6 entries");
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "init takes the addresses of 7 entries");
     return nullptr;
   }
-  void* p[6];
-  for (int i = 0; i < 6; ++i) {
+  void* p[7];
+  for (int i = 0; i < 7; ++i) {
     p[i] = PyLong_AsVoidPtr(args[i]);
     if (PyErr_Occurred()) return nullptr;
   }
@@ -44,6 +46,7 @@ PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   f_attn = reinterpret_cast<decltype(f_attn)>(p[3]);
   f_splits = reinterpret_cast<decltype(f_splits)>(p[4]);
   f_workspace = reinterpret_cast<decltype(f_workspace)>(p[5]);
+  f_copy = reinterpret_cast<decltype(f_copy)>(p[6]);
   Py_RETURN_NONE;
 }
 
@@ -244,8 +247,37 @@ PyObject* paged_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// page_copy(pool with layers: (k, k_amax, v, v_amax, pages, heads, layers, bytes and floats of a layer), device, src, dst): 0
+PyObject* page_copy(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !PyList_CheckExact(args[2]) || !PyList_CheckExact(args[3])) Py_RETURN_NONE;
+  PyObject* o = args[0];
+  const int dev = static_cast<int>(PyLong_AsLong(args[1]));
+  const Py_ssize_t m = PyList_GET_SIZE(args[2]);
+  const int64_t pages = integer(o, 4);
+  if (dev != c10::cuda::current_device() || PyList_GET_SIZE(args[3]) != m || m == 0 || m > pages) Py_RETURN_NONE;
+  std::vector<int32_t> ids(2 * m);
+  std::vector<uint8_t> role(static_cast<size_t>(pages), 0);              // 1: read, 2: written
+  for (Py_ssize_t i = 0; i < 2 * m; ++i) {
+    PyObject* v = PyList_GET_ITEM(args[i < m ? 2 : 3], i < m ? i : i - m);
+    if (!PyLong_CheckExact(v)) Py_RETURN_NONE;
+    const long long id = PyLong_AsLongLong(v);
+    if (id == -1 && PyErr_Occurred()) PyErr_Clear();
+    if (id < 0 || id >= pages) Py_RETURN_NONE;
+    uint8_t& r = role[static_cast<size_t>(id)];
+    if (i < m ? false : r != 0) Py_RETURN_NONE;                          // written twice, or read as well
+    r = i < m ? 1 : 2;
+    ids[i] = static_cast<int32_t>(id);
+  }
+  const int rc = f_copy(address(o, 0), static_cast<float*>(address(o, 1)), address(o, 2), static_cast<float*>(address(o, 3)),
+                        pages, int(integer(o, 5)), int(integer(o, 6)), integer(o, 7), integer(o, 8), ids.data(),
+                        ids.data() + m, int(m), stream_of(dev));
+  return PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(init), FAST(rope), FAST(page_write), FAST(page_read), FAST(paged_attn),
+PyMethodDef methods[] = {FAST(init), FAST(rope), FAST(page_write), FAST(page_read), FAST(page_copy), FAST(paged_attn),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torchcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -120,7 +120,7 @@ def fast():
                               f"lingbot_b200.build` ({e})") from e
         _torchcall.init(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in
                           ("lbq_rope", "lbq_page_write", "lbq_page_read", "lbq_paged_attn", "lbq_paged_attn_splits",
-                           "lbq_paged_attn_workspace")))
+                           "lbq_paged_attn_workspace", "lbq_page_copy")))
         _fast = _torchcall
     return _fast
 

@@ -57,6 +57,9 @@ class Pages:
         self.device = dev
         self._dev = k.get_device()
         self.heads = k.shape[-3]
+        layers, n = (k.shape[0] if k.dim() == 5 else 1), k.shape[-4] * self.heads
+        self._copy_args = (k.data_ptr(), ka.data_ptr(), v.data_ptr(), va.data_ptr(), k.shape[-4], self.heads, layers,
+                           n * PAGE * HEAD_DIM, n)
         self._args = None if k.dim() == 5 else (k.data_ptr(), ka.data_ptr(), v.data_ptr(), va.data_ptr(), k.shape[0],
                                                 self.heads, FORMATS[k.dtype])
 
@@ -271,6 +274,10 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
 def copy_pages(pages: Pages, src, dst):
     """Copies page src[i] to dst[i] (host sequences of ints) in every layer of the pool. All pages named by dst are
     different and none of them is a source."""
+    r = _lib.fast().page_copy(pages._copy_args, pages._dev, src, dst) if pages is not None else None
+    if r is not None:
+        _lib.check("lbq_page_copy", r)
+        return
     src, dst = array("i", src), array("i", dst)
     if len(src) != len(dst):
         raise ValueError(f"{len(src)} source pages, {len(dst)} destinations")
@@ -281,13 +288,7 @@ def copy_pages(pages: Pages, src, dst):
         raise ValueError("a page is written twice")
     if not to.isdisjoint(src):
         raise ValueError("a page is both read and written")
-    k = pages.k
-    layers = k.shape[0] if k.dim() == 5 else 1
-    num_pages, heads = k.shape[-4], k.shape[-3]
-    n = num_pages * heads
-    _lib.call_on(k.device, "lbq_page_copy", k.data_ptr(), pages.k_amax.data_ptr(), pages.v.data_ptr(),
-                 pages.v_amax.data_ptr(), num_pages, heads, layers, n * PAGE * HEAD_DIM, n, src.buffer_info()[0],
-                 dst.buffer_info()[0], len(src))
+    _lib.call_on(pages.device, "lbq_page_copy", *pages._copy_args, src.buffer_info()[0], dst.buffer_info()[0], len(src))
 
 
 @dataclass
