@@ -256,20 +256,19 @@ int lbq_page_copy(void* k_pages, float* k_amax, void* v_pages, float* v_amax, in
   return LBQ_OK;
 }
 
-int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t max_kv_len) {
+int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t max_kv_len, int ragged) {
   if (batch <= 0 || q_len <= 0 || heads <= 0 || group <= 0 || max_kv_len <= 0) return 1;
   const int64_t rows = int64_t(q_len) * group;
   const int tile = attn_tile_rows(rows);
   const int64_t ctas = (rows + tile - 1) / tile * heads * batch;
   const int64_t pages = (max_kv_len + lbq::kPageTokens - 1) / lbq::kPageTokens;
-  // Few rows: two CTAs an SM (296 at once), a split keeps at least 4 pages, one for each warp. From 90 CTAs on, where
-  // rounding down would leave a third of them idle, one more; up to 400, where one split each would nearly fill the GPU, two
-  // for long windows all the same, since sequences of a batch are seldom alike (measured, us, 1 / 2 / 4 splits of 256 CTAs of
-  // 8192 keys: all alike 84 / 93 / 100, lengths spread 1..8192 79 / 65 / 61; 3 / 4 / 6 of 96 ragged CTAs 25 / 22 / 19).
-  // Many rows: one CTA an SM, at least 8 pages to pay for the query tiles.
+  // Few rows: two CTAs an SM (296 at once), a split keeps at least 4 pages, one for each warp. Many rows: one CTA an SM, at
+  // least 8 pages to pay for the query tiles. Ragged batches get more and shorter splits, which balance the long sequences
+  // (measured, us: 256 CTAs of at most 8192 keys with 1 / 2 / 4 splits, all alike 84 / 93 / 100, lengths spread over 1..8192
+  // 79 / 65 / 61; 96 CTAs of at most 4100 keys with 3 / 4 / 6, ragged 25 / 22 / 19; with 3 / 4, all alike 27 / 34).
   const bool few = tile != lbq::kManyTile;
   int64_t n = (few ? 2 * 148 : 148) / ctas;
-  if (few && ctas >= 90 && ctas <= 400 && pages >= 32) n = ctas <= 148 ? n + 1 : 2;
+  if (few && ragged && pages >= 32 && ctas >= 64 && ctas <= 400) n = ctas <= 148 ? 2 * n : 2;
   const int64_t least = few ? 4 : 8;
   if (n > pages / least) n = pages / least;
   return int(n < 1 ? 1 : (n > 1024 ? 1024 : n));

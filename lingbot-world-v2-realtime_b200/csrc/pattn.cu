@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
 
   uint2 qb[kNT][8];
   float unit[kNT][2];                                    // per query column: undo the power of two, softmax scale, 1 / Q
-  int64_t limit[kNT][2];                                 // last visible key
+  int limit[kNT][2];                                     // last visible key of the split (a table has under 2^24 pages)
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
     const int r = tile * kRows + 8 * t + r0, i = r / a.group, g = r - i * a.group;
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
     for (int e = 0; e < 2; ++e) {
       unit[t][e] = __shfl_sync(0xffffffffu, u, 8 * quad + 4 * e);      // column 2 quad + e is row r0 of that lane
       const int qi = (tile * kRows + 8 * t + 2 * quad + e) / a.group;
-      limit[t][e] = (qi >= tk.qn ? -1 : (a.causal ? tk.kv - tk.qn + qi : tk.kv - 1)) - int64_t(p0) * kPageTokens;
+      limit[t][e] = qi >= tk.qn ? -1 : int((a.causal ? tk.kv - tk.qn + qi : tk.kv - 1) - int64_t(p0) * kPageTokens);
     }
   }
   float m[kNT][2], l[kNT][2], o[8][kNT][4];
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
     }
     const float kat = fmaxf(ka, kTinyScale), vat = fmaxf(va, kTinyScale);
     const float lv = __log2f(vat), iv = __frcp_rn(vat);
-    const int64_t j0 = int64_t(i) * kPageTokens;
+    const int j0 = i * kPageTokens;
     uint32_t pb[kNT][4][2];
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int64_t j = j0 + mt * 16 + r0 + 8 * (e >> 1);
+            const int j = j0 + mt * 16 + r0 + 8 * (e >> 1);
             if (!ok || j > limit[t][e & 1]) x[t][mt][e] = -INFINITY;
           }
       }
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
     }
     // rows of V past the sequence's tokens hold whatever the page held before: weight 0 times a NaN code (e4m3; int8 has
     // none) would be NaN, so they are read as 0
-    const int64_t rest = ok ? tk.kv - (int64_t(p0) * kPageTokens + j0) : 0;
+    const int rest = ok ? int(tk.kv - (int64_t(p0) * kPageTokens + j0)) : 0;
     const bool clip = kFmt == 1 && rest < kPageTokens;
     // o: rows r0 and r0 + 8 of a tile are channels 16 c + 2 r0 and 16 c + 2 r0 + 1, columns the queries
 #pragma unroll

@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
     const float unit = stage_query<kDt>(qrow, sQ + t * kQTile, rl) * a.score_log2;
     fence_proxy_async_smem();
     mbar_arrive(&sh->q_full);
-    const int64_t limit = (!on ? -1 : (a.causal ? tk.kv - tk.qn + qi : tk.kv - 1)) - int64_t(p0) * kPageTokens;
+    const int limit = !on ? -1 : int((a.causal ? tk.kv - tk.qn + qi : tk.kv - 1) - int64_t(p0) * kPageTokens);
     float m = -INFINITY, l = 0.f;
     // The scales of the next page are loaded one page ahead, its id two pages ahead. They are kept above 0 (a written
     // page's are at least 2^-40): a masked score is -inf times ka, and va is divided by.
@@ -312,9 +312,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
       tmem_ld_wait(sv0);
       reg_anchor(sv1);
       auto F = [&](int i) { return __uint_as_float(sv[i]); };
-      const int64_t rest = limit - int64_t(u) * kPageTokens;   // last visible key of the page
+      const int rest = limit - u * kPageTokens;           // last visible key of the page
       if (!__all_sync(0xffffffffu, rest >= 63 && known)) {
-        const int last = known ? int(rest < 63 ? (rest < 0 ? -1 : rest) : 63) : -1;
+        const int last = known ? min(rest, 63) : -1;
 #pragma unroll
         for (int i = 0; i < 64; ++i)
           if (i > last) sv[i] = 0xff800000u;

@@ -233,7 +233,7 @@ PyObject* paged_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (scale == -1.0 && PyErr_Occurred()) return nullptr;
   const int group = int(hq / pool.heads);
   const int64_t longest = kv ? table->size(1) * 64 : kv0;
-  const int splits = f_splits(int(b), int(lq), pool.heads, group, longest);
+  const int splits = f_splits(int(b), int(lq), pool.heads, group, longest, b > 1 && ql != nullptr);
   at::Tensor out = at::empty_like(*q), ws;
   const size_t need = f_workspace(int(b), int(lq), pool.heads, group, splits);
   if (need > 0) ws = at::empty({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));

@@ -69,7 +69,7 @@ SIGNATURES = {
     "lbq_page_read": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _i32, _vp,
                              _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp]),
     "lbq_page_copy": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _i64, _vp, _vp, _i32, _vp]),
-    "lbq_paged_attn_splits": (_i32, [_i32, _i32, _i32, _i32, _i64]),
+    "lbq_paged_attn_splits": (_i32, [_i32, _i32, _i32, _i32, _i64, _i32]),
     "lbq_paged_attn_workspace": (_sz, [_i32, _i32, _i32, _i32, _i32]),
     "lbq_paged_attn": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _i64,
                               _vp, _i32, _i32, _i32, _i32, _f32, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _sz, _i32,

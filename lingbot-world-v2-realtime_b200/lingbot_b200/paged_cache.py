@@ -258,7 +258,8 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
                 raise ValueError(f"kv_lens {k0} exceeds max_kv_len {longest}")
         lib = _lib.load()
         if num_splits is None:
-            num_splits = lib.lbq_paged_attn_splits(b, lq, heads, group, longest)
+            # a padded batch's lengths differ
+            num_splits = lib.lbq_paged_attn_splits(b, lq, heads, group, longest, int(b > 1 and q_lens is not None))
         ws, ws_bytes = None, 0
         if num_splits > 1:
             ws_bytes = lib.lbq_paged_attn_workspace(b, lq, heads, group, num_splits)

@@ -81,8 +81,8 @@ def test_c_entries_refuse_bad_arguments():
     assert attn(lq=0) == 0
     assert lib.lbq_paged_attn_workspace(1, 1, 12, 1, 1) == 0
     assert lib.lbq_paged_attn_workspace(1, 1, 12, 1, 4) >= 4 * 12 * 130 * 4
-    assert lib.lbq_paged_attn_splits(1, 1, 12, 1, 1) == 1
-    assert lib.lbq_paged_attn_splits(1, 1, 12, 1, 30160) > 1
+    assert lib.lbq_paged_attn_splits(1, 1, 12, 1, 1, 0) == 1
+    assert lib.lbq_paged_attn_splits(1, 1, 12, 1, 30160, 0) > 1
 
     def write(**kw):
         a = dict(k=p, start=None, s0=0, l=8, cos=None, sin=None, rs=0, rr=0, rot=0, inter=1)
