@@ -79,6 +79,15 @@ int finish(cudaError_t e, const char* what) {
 constexpr int64_t kFewRows = 64;
 int attn_tile_rows(int64_t rows) { return rows <= 8 ? 8 : (rows <= kFewRows ? 16 : lbq::kManyTile); }
 
+// Key splits that fit the GPU at once (two CTAs an SM) and are at most 8 are one cluster, which merges them itself: no
+// workspace, no second launch (one token against 1000 keys x 12 heads, 4 splits: 6.9 against 7.5 us). CTAs of several waves
+// are left to be scheduled one by one (256 CTAs of ragged lengths, 2 splits: 65 us, as clusters 78).
+constexpr int64_t kFewCtas = 2 * 148;
+bool attn_clustered(int64_t rows, int heads, int batch, int splits) {
+  const int tile = attn_tile_rows(rows);
+  return tile != lbq::kManyTile && splits > 1 && splits <= 8 && (rows + tile - 1) / tile * heads * batch * splits <= kFewCtas;
+}
+
 }  // namespace
 
 extern "C" {
@@ -267,10 +276,11 @@ int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t ma
   // (measured, us: 256 CTAs of at most 8192 keys with 1 / 2 / 4 splits, all alike 84 / 93 / 100, lengths spread over 1..8192
   // 79 / 65 / 61; 96 CTAs of at most 4100 keys with 3 / 4 / 6, ragged 25 / 22 / 19; with 3 / 4, all alike 27 / 34).
   const bool few = tile != lbq::kManyTile;
-  int64_t n = (few ? 2 * 148 : 148) / ctas;
+  int64_t n = (few ? kFewCtas : 148) / ctas;
   if (few && ragged && pages >= 32 && ctas >= 64 && ctas <= 400) n = ctas <= 148 ? 2 * n : 2;
   const int64_t least = few ? 4 : 8;
   if (n > pages / least) n = pages / least;
+  if (few && n > 8 && n <= 16 && pages <= 96) n = 8;      // one cluster's worth: no merge launch (16 splits of 64 pages: alike)
   return int(n < 1 ? 1 : (n > 1024 ? 1024 : n));
 }
 
@@ -278,6 +288,7 @@ size_t lbq_paged_attn_workspace(int batch, int q_len, int heads, int group, int 
   if (batch <= 0 || q_len < 0 || heads <= 0 || group <= 0 || num_splits <= 1) return 0;
   const uint64_t rows = uint64_t(q_len) * group;
   const uint64_t tile = attn_tile_rows(int64_t(rows));
+  if (attn_clustered(int64_t(rows), heads, batch, num_splits)) return 0;
   uint64_t n, bytes;
   if (__builtin_mul_overflow((rows + tile - 1) / tile * tile, uint64_t(batch) * heads, &n) ||
       __builtin_mul_overflow(n, uint64_t(num_splits), &n) || __builtin_mul_overflow(n, uint64_t(128 * 4 + 8), &bytes))
@@ -315,7 +326,8 @@ int lbq_paged_attn(const void* q, int64_t sq_b, int64_t sq_l, int64_t sq_h, cons
   a.split_pages = (pages + num_splits - 1) / num_splits;
   a.splits = (pages + a.split_pages - 1) / a.split_pages;
   if (a.splits > kMaxGrid) return set_error(LBQ_ERR_ARG, "too many key splits");
-  if (a.splits > 1) {
+  a.clustered = attn_clustered(rows, heads, batch, a.splits);
+  if (a.splits > 1 && !a.clustered) {
     const size_t need = lbq_paged_attn_workspace(batch, q_len, heads, group, a.splits);
     if (workspace == nullptr || workspace_bytes < need)
       return set_error(LBQ_ERR_ARG, "workspace of %zu bytes is smaller than the %zu needed", workspace_bytes, need);
@@ -364,7 +376,7 @@ int lbq_paged_attn(const void* q, int64_t sq_b, int64_t sq_l, int64_t sq_h, cons
     r = finish(lbq::launch_paged_rows(a, st), "paged_attn launch");
   }
   if (r) return r;
-  if (a.splits > 1) return finish(lbq::launch_paged_combine(a, st), "paged_attn merge launch");
+  if (a.splits > 1 && !a.clustered) return finish(lbq::launch_paged_combine(a, st), "paged_attn merge launch");
   return LBQ_OK;
 }
 

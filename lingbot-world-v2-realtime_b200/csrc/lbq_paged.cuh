@@ -67,18 +67,28 @@ __device__ __forceinline__ float natural_lse(float m, float l) {
 }
 
 template <class... Params, class... Args>
-cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+cudaError_t launch_after_clustered(void (*kernel)(Params...), dim3 cluster, dim3 grid, dim3 block, size_t smem,
+                                   cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster.x;
+  at[1].val.clusterDim.y = cluster.y;
+  at[1].val.clusterDim.z = cluster.z;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
+template <class... Params, class... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+  return launch_after_clustered(kernel, dim3(1), grid, block, smem, st, args...);
 }
 
 }  // namespace lbq

@@ -108,7 +108,8 @@ struct PagedAttnArgs {
   float v_unit;                 // 1 / Q
   int tile_rows, tiles;         // rows (query token, query head of the K/V head) of a CTA, tiles of a K/V head
   int splits, split_pages;      // key splits, and the pages of one
-  float* o_part;                // [splits][batch * heads][tiles * tile_rows][128] (splits > 1)
+  int clustered;                // the splits of a tile are one cluster, which merges them (few rows, at most 8 splits)
+  float* o_part;                // [splits][batch * heads][tiles * tile_rows][128] (splits > 1, not clustered)
   float2* ml_part;              // the same rows' (max in log2 units, sum)
   int wide_out;                 // out's base and strides are 32-byte aligned
   int* status;

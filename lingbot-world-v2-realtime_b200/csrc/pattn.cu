@@ -35,7 +35,7 @@ constexpr int kDecWarps = 4;
 constexpr int kDecSlots = 6;
 constexpr int kMergePitch = 132;                       // floats of a merged row in shared memory
 constexpr size_t kDecSmem = 1024 + size_t(kDecSlots) * 2 * kPageBytes;
-static_assert(size_t(kDecWarps) * 16 * kMergePitch * 4 <= size_t(kDecSlots) * 2 * kPageBytes, "merge area");
+static_assert(size_t(kDecWarps * kMergePitch + 128) * 16 * 4 <= size_t(kDecSlots) * 2 * kPageBytes, "merge area");
 
 // Volatile, so that they stay between the wait for a slot and its refill; not the products, which may move freely.
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -98,6 +98,20 @@ __device__ __forceinline__ float load_query(const uint16_t* row, int quad, uint2
   }
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The float(s) at `p` of CTA `rank` of the cluster.
+__device__ __forceinline__ float2 peer_f2(const float* p, int rank) {
+  float2 v;
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [ra];\n\t}"
+      : "=f"(v.x), "=f"(v.y)
+      : "r"(smem_u32(p)), "r"(rank)
+      : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void st_release(int* p, int v) {
   asm volatile("st.release.cta.shared.s32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
 }
@@ -113,6 +127,7 @@ struct DecShared {
   int abort;
   float m[kDecWarps][16];
   float l[kDecWarps][16];
+  float2 ml[16];                                         // clustered splits: this CTA's maximum and sum of each row
 };
 
 template <int kFmt, int kDt, int kNT>
@@ -138,8 +153,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
   const TileKeys tk = tile_keys(a, b, tile);
   const int pages = int((tk.visible + kPageTokens - 1) / kPageTokens);
   const int n = max(0, min(pages - p0, a.split_pages));
-  if (split > 0 && n == 0) return;
-  const bool single = pages <= a.split_pages;
+  const bool single = pages <= a.split_pages;            // of the whole tile, so of every CTA of its cluster
+  if (split > 0 && (single || (n == 0 && !a.clustered))) return;
   const uint32_t pool = uint32_t(a.pt.num_pages);
 
   // Page ids are loaded well before they are looked at. One outside the pool is recorded, and read as page 0 with every
@@ -356,11 +371,13 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
     va = va_next;
   }
   __syncthreads();
-  if (*abort_flag) {                                       // let copies in flight land before the CTA goes away
+  const bool aborted = *abort_flag;
+  if (aborted) {                                           // let copies in flight land before the CTA goes away
     if (threadIdx.x == 0)
       for (int s = 0; s < kDecSlots; ++s)
         if (sh.issued[s]) mbar_drain_wait(&sh.full[s], (sh.issued[s] - 1) & 1);
-    return;
+    if (single || !a.clustered) return;
+    __syncthreads();                                       // the cluster's other CTAs wait for this one
   }
 
   // merge the warps: rows of 128 channels in the ring, which nothing reads any more
@@ -419,6 +436,12 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
         if (a.lse && seg == 0) a.lse[(int64_t(b) * a.q_len + qi) * (a.heads * a.group) + head] = natural_lse(mm - kWeightBits, ll);
       }
+    } else if (a.clustered) {
+      // this split's row, unscaled, behind the merge area
+      float* p = mo + kDecWarps * kRows * kMergePitch + rr * 128 + 8 * seg;
+      *reinterpret_cast<float4*>(p) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(p + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (seg == 0) sh.ml[rr] = make_float2(mm, ll);
     } else {
       const int64_t at = (int64_t(split) * a.batch * a.heads + int64_t(b) * a.heads + h) * (int64_t(a.tiles) * a.tile_rows) + row;
       float4* p = reinterpret_cast<float4*>(a.o_part + at * 128 + 8 * seg);
@@ -427,6 +450,43 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
       if (seg == 0) a.ml_part[at] = make_float2(mm - kWeightBits, ll);
     }
   }
+  if (single || !a.clustered) return;
+  // The cluster's CTAs share the rows out, two at a time with two channels a thread, and read one another's splits.
+  cluster_sync();
+  const int ch = 2 * (threadIdx.x & 63);
+  for (int rr = 2 * split + (threadIdx.x >> 6); rr < kRows; rr += 2 * a.splits) {
+    const int row = tile * kRows + rr, qi = row / a.group, head = h * a.group + (row - qi * a.group);
+    float2 ml[8], x[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      ml[s] = make_float2(-INFINITY, 0.f);
+      x[s] = make_float2(0.f, 0.f);
+      if (s < a.splits) {
+        ml[s] = peer_f2(&sh.ml[rr].x, s);
+        x[s] = peer_f2(mo + kDecWarps * kRows * kMergePitch + rr * 128 + ch, s);
+      }
+    }
+    float mm = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) mm = fmaxf(mm, ml[s].x);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    float2 o2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float f = ex2_approx(ml[s].x - ref);
+      ll += ml[s].y * f;
+      o2.x += x[s].x * f;
+      o2.y += x[s].y * f;
+    }
+    if (qi < a.q_len) {
+      const float inv = ll == 0.f ? 0.f : a.v_unit / ll;
+      uint16_t* p = static_cast<uint16_t*>(a.out) + b * a.so[0] + qi * a.so[1] + head * a.so[2] + ch;
+      *reinterpret_cast<uint32_t*>(p) = ll == 0.f ? 0u : pack_act2(o2.x * inv, o2.y * inv, kDt);
+      if (a.lse && ch == 0) a.lse[(int64_t(b) * a.q_len + qi) * (a.heads * a.group) + head] = natural_lse(mm - kWeightBits, ll);
+    }
+  }
+  cluster_sync();                                          // nobody reads this CTA's memory any more
 }
 
 // Merge of the key splits: one CTA a row, its 4 warps take the splits in turn, 4 channels a lane. A split's weight is
@@ -512,7 +572,8 @@ template <int kFmt, int kDt, int kNT>
 cudaError_t launch_decode_as(const PagedAttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
   if (cudaError_t e = allow_dynamic_smem<paged_decode_kernel<kFmt, kDt, kNT>>(int(kDecSmem)); e != cudaSuccess) return e;
   const dim3 grid(unsigned(a.heads) * a.tiles, a.splits, a.batch);
-  return launch_after(paged_decode_kernel<kFmt, kDt, kNT>, grid, dim3(kDecWarps * 32), kDecSmem, st, tm_k, tm_v, a);
+  return launch_after_clustered(paged_decode_kernel<kFmt, kDt, kNT>, dim3(1, a.clustered ? a.splits : 1), grid,
+                                dim3(kDecWarps * 32), kDecSmem, st, tm_k, tm_v, a);
 }
 template <int kFmt, int kDt>
 cudaError_t launch_decode_rows(const PagedAttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {

@@ -75,12 +75,16 @@ def test_c_entries_refuse_bad_arguments():
                                   a["splits"], a["ws"], a["wsb"], 0, None)
     for kw, rc, word in [(dict(q=None), 1, b"null"), (dict(out=p + 8), 2, b"aligned"), (dict(kv0=257), 1, b"kv_len"),
                          (dict(kv0=-1), 1, b"kv_len"), (dict(group=0), 1, b"group"), (dict(b=70000), 1, b"batch"),
-                         (dict(splits=2), 1, b"workspace"), (dict(splits=2, ws=p, wsb=8), 1, b"workspace"),
+                         (dict(splits=9, kv0=1152, width=18), 1, b"workspace"),
+                         (dict(splits=9, kv0=1152, width=18, ws=p, wsb=8), 1, b"workspace"),
                          (dict(lq=1 << 28, group=5), 1, b"large")]:
         assert attn(**kw) == rc and word in err(), (kw, err())
     assert attn(lq=0) == 0
     assert lib.lbq_paged_attn_workspace(1, 1, 12, 1, 1) == 0
-    assert lib.lbq_paged_attn_workspace(1, 1, 12, 1, 4) >= 4 * 12 * 130 * 4
+    assert lib.lbq_paged_attn_workspace(1, 1, 12, 1, 8) == 0          # one cluster
+    assert lib.lbq_paged_attn_workspace(4, 1, 12, 1, 8) > 0           # more CTAs than the GPU holds at once
+    assert lib.lbq_paged_attn_workspace(1, 1, 12, 1, 9) >= 9 * 12 * 130 * 4
+    assert lib.lbq_paged_attn_workspace(1, 100, 12, 1, 2) >= 2 * 12 * 100 * 130 * 4
     assert lib.lbq_paged_attn_splits(1, 1, 12, 1, 1, 0) == 1
     assert lib.lbq_paged_attn_splits(1, 1, 12, 1, 30160, 0) > 1
 
