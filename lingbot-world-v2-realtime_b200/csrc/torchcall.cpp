@@ -71,6 +71,13 @@ bool table_ok(const at::Tensor& t, int dev, int64_t batch) {
   return t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == batch && t.size(1) > 0 && t.is_cuda() &&
          t.get_device() == dev && (t.stride(1) == 1 || t.size(1) == 1);
 }
+// A Python int that fits 64 bits and is not negative.
+bool whole(PyObject* o, int64_t* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  *v = PyLong_AsLongLong(o);
+  if (*v == -1 && PyErr_Occurred()) PyErr_Clear();
+  return *v >= 0;
+}
 // A count of every sequence: int32 [batch] tensor or a non-negative int.
 bool count(PyObject* o, int dev, int64_t batch, const int32_t** p, int64_t* v) {
   *p = nullptr;
@@ -80,10 +87,7 @@ bool count(PyObject* o, int dev, int64_t batch, const int32_t** p, int64_t* v) {
     *p = t->const_data_ptr<int32_t>();
     return true;
   }
-  if (!PyLong_CheckExact(o)) return false;
-  *v = PyLong_AsLongLong(o);
-  if (*v == -1 && PyErr_Occurred()) PyErr_Clear();
-  return *v >= 0;
+  return whole(o, v);
 }
 struct Positions {
   const void* p = nullptr;
@@ -115,8 +119,8 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
                        k->size(3) != x->size(3)))
     Py_RETURN_NONE;
   Positions pos;
-  if (!positions(args[4], dev, b, l, &pos) || !PyLong_CheckExact(args[5])) Py_RETURN_NONE;
-  const int64_t start = PyLong_AsLongLong(args[5]);
+  int64_t start;
+  if (!positions(args[4], dev, b, l, &pos) || !whole(args[5], &start)) Py_RETURN_NONE;
   const int inverse = PyObject_IsTrue(args[6]);
   PyObject* r = args[2];
   at::Tensor y = at::empty_like(*x), z;
@@ -185,12 +189,13 @@ PyObject* page_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // page_read(pool, device, table, start, length, dtype code, lens or None): (k, v)
 PyObject* page_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 7 || !PyTuple_CheckExact(args[0]) || !PyLong_CheckExact(args[4])) Py_RETURN_NONE;
+  int64_t length;
+  if (n != 7 || !PyTuple_CheckExact(args[0]) || !whole(args[4], &length)) Py_RETURN_NONE;
   const Pool pool(args[0]);
   const int dev = static_cast<int>(PyLong_AsLong(args[1]));
   const at::Tensor* table = tensor(args[2]);
   if (dev != c10::cuda::current_device() || !table || table->dim() != 2) Py_RETURN_NONE;
-  const int64_t b = table->size(0), length = PyLong_AsLongLong(args[4]);
+  const int64_t b = table->size(0);
   const int dt = static_cast<int>(PyLong_AsLong(args[5]));
   if (b <= 0 || length <= 0 || length > (1 << 28) || !table_ok(*table, dev, b)) Py_RETURN_NONE;
   const int32_t *start, *lens = nullptr;

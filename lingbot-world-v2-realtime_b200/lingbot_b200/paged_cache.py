@@ -108,6 +108,8 @@ def _counts(name, t, batch, device):
     t = int(t)
     if t < 0:
         raise ValueError(f"{name} {t} is negative")
+    if t >= 1 << 62:                                             # ctypes would drop the upper bits
+        raise ValueError(f"{name} {t} does not fit 64 bits")
     return None, t
 
 
@@ -118,6 +120,17 @@ def _check_rows(name, x, device):
         raise ValueError(f"{name} must be [B, L, heads, {HEAD_DIM}] with unit channel stride, got {tuple(x.shape)}")
     if x.device != device:
         raise ValueError(f"{name} on {x.device}, pages on {device}")
+
+
+def _overlap(a, b):
+    """Whether the address ranges of two tensors meet."""
+    def span(t):
+        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
 
 
 def _no_grad():
@@ -240,6 +253,10 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
         _check_rows("out", out, dev)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
+        if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+            raise ValueError("out has elements that share memory")
+        if (out.data_ptr() != q.data_ptr() or out.stride() != q.stride()) and _overlap(out, q):
+            raise ValueError("out overlaps q without being it")
     lse = torch.empty((b, lq, hq), dtype=torch.float32, device=dev) if return_lse else None
     if b and lq:
         tp, ts, width = _table(page_table, b, dev)
@@ -318,7 +335,7 @@ class PagedCache:
         self.max_pages = int(max_pages)
         self._free = list(range(self.num_pages - 1, -1, -1))      # ascending ids are taken first
         self._refs = [0] * self.num_pages
-        self._sessions = {}                                       # id -> [pages, tokens, version]
+        self._sessions = {}                                       # id -> [pages, tokens, version, evicted tokens]
         self._next = 0
         self._version = 0
 
@@ -358,21 +375,21 @@ class PagedCache:
         """A new, empty session."""
         return self._add([], 0)
 
-    def _add(self, pages, tokens):
+    def _add(self, pages, tokens, evicted=0):
         self._version += 1
-        self._sessions[self._next] = [pages, tokens, self._version]
+        self._sessions[self._next] = [pages, tokens, self._version, evicted]
         self._next += 1
         return self._next - 1
 
     def fork(self, session):
         """A new session with the same committed tokens. Their pages are shared; an unfinished last page is copied when
         one of the sessions is next planned to write into it. Plans of `session` made before end."""
-        pages, tokens, _ = self._get(session)
+        pages, tokens, _, evicted = self._get(session)
         pages = pages[:(tokens + PAGE - 1) // PAGE]
         for p in pages:
             self._refs[p] += 1
         self._touch(session)
-        return self._add(pages, tokens)
+        return self._add(pages, tokens, evicted)
 
     def close(self, session):
         """Ends a session and frees the pages that no other session holds."""
@@ -393,11 +410,12 @@ class PagedCache:
             raise ValueError("a session is planned twice")
         if min(new) < 0:
             raise ValueError("negative token count")
-        if into is not None and len(into.sessions) != len(sessions):
-            raise ValueError(f"a plan of {len(into.sessions)} sessions cannot take {len(sessions)}")
+        if into is not None and tuple(into.table.shape) != (len(sessions), self.max_pages):
+            raise ValueError(f"a plan whose table is {tuple(into.table.shape)} cannot take {len(sessions)} sessions of "
+                             f"{self.max_pages} pages: make it with fixed_plan")
         need, refs, copies = 0, {}, []
         for s, n in zip(sessions, new):
-            pages, tokens, _ = self._get(s)
+            pages, tokens = self._get(s)[:2]
             total = (tokens + n + PAGE - 1) // PAGE
             if total > self.max_pages:
                 raise ValueError(f"session {s}: {tokens + n} tokens exceed {self.max_pages} pages")
@@ -422,7 +440,7 @@ class PagedCache:
                 self._touch(s)
             copy_pages(self.pages, src, dst)
         for s, n in zip(sessions, new):
-            pages, tokens, _ = self._sessions[s]
+            pages, tokens = self._sessions[s][:2]
             while len(pages) * PAGE < tokens + n:
                 pages.append(self._take())
         held = [self._sessions[s][1] for s in sessions]
@@ -435,9 +453,6 @@ class PagedCache:
         if into is None:
             table, counts = table.to(dev), counts.to(dev)
             return Plan(sessions, new, held, table, counts[0], counts[1], counts[2], versions)
-        if tuple(into.table.shape) != tuple(table.shape):
-            raise ValueError(f"the plan's table is {tuple(into.table.shape)}, not {tuple(table.shape)}: make it with "
-                             "fixed_plan")
         into.table.copy_(table)
         for t, c in zip((into.start, into.lens, into.kv_lens), counts):
             t.copy_(c)
@@ -465,6 +480,8 @@ class PagedCache:
         self._check(plan)
         if k.dim() == 4 and k.shape[1] < max(plan.new):
             raise ValueError(f"{k.shape[1]} tokens given, {max(plan.new)} planned")
+        if rope is not None and positions is None and any(self._sessions[s][3] for s in plan.sessions):
+            raise ValueError("tokens were evicted from a session of this plan: pass the new tokens' positions")
         write(self.layers[layer], plan.table, plan.start, k, v, lens=plan.lens, rope=rope, positions=positions)
 
     def attend(self, layer, plan: Plan, q, causal=False, sm_scale=None, out=None, return_lse=False):
@@ -484,15 +501,17 @@ class PagedCache:
 
     def evict(self, session, sink_tokens, evicted):
         """Drops `evicted` tokens after the first `sink_tokens` (both multiples of 64): their pages leave the session's
-        table, nothing is copied. Later tokens keep their K as it was roped."""
+        table, nothing is copied. The tokens that stay keep their K as it was roped; `write` with rope then wants
+        positions, since a token's index in the session is no longer its position."""
         if sink_tokens % PAGE or evicted % PAGE or sink_tokens < 0 or evicted < 0:
             raise ValueError(f"sink {sink_tokens} and evicted {evicted} must be non-negative multiples of {PAGE}")
-        pages, tokens, _ = self._get(session)
+        pages, tokens = self._get(session)[:2]
         if sink_tokens + evicted > tokens:
             raise ValueError(f"session {session} holds {tokens} tokens, fewer than {sink_tokens} + {evicted}")
         a, b = sink_tokens // PAGE, (sink_tokens + evicted) // PAGE
         gone = pages[a:b]
         self._sessions[session][:2] = pages[:a] + pages[b:], tokens - evicted
+        self._sessions[session][3] += evicted
         self._touch(session)
         for p in gone:
             self._drop(p)

@@ -132,6 +132,9 @@ def apply(x, rope: Rope, positions=None, start=0, inverse=False, out=None, k=Non
         if torch.is_grad_enabled():
             raise RuntimeError("rope.apply records no gradient: call it under torch.no_grad(), and rotate the gradient "
                                "back with inverse=True")
+    start = int(start)
+    if not 0 <= start < 1 << 62:
+        raise ValueError(f"start {start} must be a non-negative 64-bit position")
     if (out is None) != (k_out is None) and k is not None:
         raise ValueError("out and k_out: give both or neither")
     if out is None:
@@ -144,7 +147,7 @@ def apply(x, rope: Rope, positions=None, start=0, inverse=False, out=None, k=Non
     if k is None:
         if b and l and h:
             _lib.call_on(dev, "lbq_rope", x.data_ptr(), sx[0], sx[1], sx[2], y.data_ptr(), sy[0], sy[1], sy[2], h, None, 0, 0,
-                         0, None, 0, 0, 0, 0, b, l, d, *table, int(start), 1 if inverse else 0, _DTYPES[x.dtype])
+                         0, None, 0, 0, 0, 0, b, l, d, *table, start, 1 if inverse else 0, _DTYPES[x.dtype])
         return y
     _check("k", k)
     kb, kl, hk, kd = k.shape
@@ -162,6 +165,6 @@ def apply(x, rope: Rope, positions=None, start=0, inverse=False, out=None, k=Non
     if b and l:
         sk, sz = k.stride(), z.stride()
         _lib.call_on(dev, "lbq_rope", x.data_ptr(), sx[0], sx[1], sx[2], y.data_ptr(), sy[0], sy[1], sy[2], h, k.data_ptr(),
-                     sk[0], sk[1], sk[2], z.data_ptr(), sz[0], sz[1], sz[2], hk, b, l, d, *table, int(start),
+                     sk[0], sk[1], sk[2], z.data_ptr(), sz[0], sz[1], sz[2], hk, b, l, d, *table, start,
                      1 if inverse else 0, _DTYPES[x.dtype])
     return y, z

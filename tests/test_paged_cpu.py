@@ -74,7 +74,7 @@ def test_c_entries_refuse_bad_arguments():
                                   a["kv0"], None, a["b"], a["lq"], a["group"], 0, 0.0, a["out"], 1024, 128, 128, None,
                                   a["splits"], a["ws"], a["wsb"], 0, None)
     for kw, rc, word in [(dict(q=None), 1, b"null"), (dict(out=p + 8), 2, b"aligned"), (dict(kv0=257), 1, b"kv_len"),
-                         (dict(kv0=-1), 1, b"kv_len"), (dict(group=0), 1, b"group"), (dict(b=70000), 1, b"batch"),
+                         (dict(kv0=-1), 1, b"kv_len"), (dict(group=0), 1, b"group"), (dict(group=1 << 25), 1, b"group"), (dict(b=70000), 1, b"batch"),
                          (dict(splits=9, kv0=1152, width=18), 1, b"workspace"),
                          (dict(splits=9, kv0=1152, width=18, ws=p, wsb=8), 1, b"workspace"),
                          (dict(lq=1 << 28, group=5), 1, b"large")]:
@@ -230,8 +230,16 @@ def test_stale_plans_and_bad_calls_are_refused(monkeypatch):
     table = fixed.table
     got = c.plan([b], 60, into=fixed)
     assert got is fixed and fixed.table is table and int(fixed.kv_lens[0]) == c.tokens(b) + 60
+    before = (c.free_pages, c.page_ids(a), c.page_ids(b))
     with pytest.raises(ValueError, match="cannot take"):
-        c.plan([a, b], 1, into=fixed)
+        c.plan([a, b], 100, into=fixed)
+    with pytest.raises(ValueError, match="fixed_plan"):
+        c.plan([b], 100, into=c.plan([b], 1))
+    assert before == (c.free_pages, c.page_ids(a), c.page_ids(b))
+    r = type("R", (), {})()
+    k = torch.zeros(1, 60, 1, 128)
+    with pytest.raises(ValueError, match="positions"):                # 64 tokens of b were evicted
+        c.write(0, fixed, k, k, rope=r)
 
 
 def test_copy_pages_refuses_overlap():

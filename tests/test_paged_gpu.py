@@ -352,6 +352,90 @@ def test_streams_graphs_and_gradients():
         pc.attend(qs[0].clone().requires_grad_(), p, table, lens)
 
 
+def test_refusals():
+    from lingbot_b200 import paged_cache as pc, rope
+    p = pool(P.make_pages(8, 4, 2, torch.int8))
+    table, lens = i32([[0, 1], [2, 3]]), i32([100, 128])
+    q = torch.randn(2, 3, 4, 128).bfloat16().cuda()
+    big = 1 << 70
+    for exc, word, call in [
+            (ValueError, "multiple", lambda: pc.attend(q[:, :, :3], p, table, lens)),
+            (TypeError, "q must be", lambda: pc.attend(q.float(), p, table, lens)),
+            (ValueError, "pages on", lambda: pc.attend(q.cpu(), p, table, lens)),
+            (ValueError, "page table", lambda: pc.attend(q, p, table.long(), lens)),
+            (ValueError, "page table", lambda: pc.attend(q, p, table[:1], lens)),
+            (ValueError, "page table", lambda: pc.attend(q, p, table.cpu(), lens)),
+            (ValueError, "kv_lens", lambda: pc.attend(q, p, table, lens.long())),
+            (ValueError, "negative", lambda: pc.attend(q, p, table, -1)),
+            (Exception, "outside", lambda: pc.attend(q, p, table, 129)),
+            (TypeError, "q_lens", lambda: pc.attend(q, p, table, lens, q_lens=3)),
+            (ValueError, "exceeds", lambda: pc.attend(q, p, table, 100, max_kv_len=99)),
+            (ValueError, "overlaps", lambda: pc.attend(q[:, :2], p, table, lens, out=q[:, 1:])),
+            (ValueError, "share memory", lambda: pc.attend(q, p, table, lens, out=torch.empty_like(q)[:, :1].expand(q.shape))),
+            (ValueError, "heads", lambda: pc.write(p, table, 0, q, q)),
+            (ValueError, "differ", lambda: pc.write(p, table, 0, q[:, :, :2], q[:, :2, :2])),
+            (ValueError, "positions", lambda: pc.write(p, table, 0, q[:, :, :2], q[:, :, :2], positions=lens)),
+            (ValueError, "of 3 tokens", lambda: pc.write(p, table, 0, q[:, :, :2], q[:, :, :2], lens=4)),
+            (Exception, "outside", lambda: pc.write(p, table, 126, q[:, :, :2], q[:, :, :2])),
+            (RuntimeError, "gradient", lambda: pc.write(p, table, 0, q[:, :, :2].clone().requires_grad_(), q[:, :, :2])),
+            (Exception, "outside", lambda: pc.window(p, table, 100, 29)),
+            (ValueError, "negative", lambda: pc.window(p, table, 0, -1)),
+            (TypeError, "dtype", lambda: pc.window(p, table, 0, 1, torch.float32)),
+            (ValueError, "twice", lambda: pc.copy_pages(p, [0, 1], [2, 2])),
+            (ValueError, "both", lambda: pc.copy_pages(p, [0, 1], [1, 2])),
+            (Exception, "outside", lambda: pc.copy_pages(p, [0], [4])),
+            (Exception, "outside", lambda: pc.copy_pages(p, [-1], [3])),
+            (Exception, None, lambda: pc.window(p, table, 0, big)),
+            (ValueError, "64 bits", lambda: pc.window(p, table, big, 1)),
+            (ValueError, "start", lambda: rope.apply(q, rope.tables(8, 64), start=big)),
+            (ValueError, "start", lambda: rope.apply(q, rope.tables(8, 64), start=-1))]:
+        with pytest.raises(exc, match=word):
+            call()
+    # in place, lengths as ints, nothing to do
+    want = pc.attend(q, p, table, 128)
+    x = q.clone()
+    assert pc.attend(x, p, table, 128, out=x).data_ptr() == x.data_ptr() and torch.equal(x, want)
+    assert torch.equal(pc.attend(q, p, table, i32([128, 128]), return_lse=True)[0], want)
+    assert pc.attend(q[:0], p, table[:0], lens[:0]).shape == (0, 3, 4, 128)
+    assert pc.attend(q[:, :0], p, table, lens).shape == (2, 0, 4, 128)
+    before = p.k.clone()
+    pc.write(p, table, 0, q[:, :0, :2], q[:, :0, :2])
+    pc.write(p, table, 0, q[:, :, :2], q[:, :, :2], lens=0)
+    pc.copy_pages(p, [], [])
+    assert torch.equal(raw(p.k), raw(before))
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    """Nothing needs a call outside a capture first."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from lingbot_b200 import paged_cache as pc, rope, _lib
+p = pc.alloc_pages(8, 2, "cuda")
+t = rope.tables(200, 128)
+table = torch.tensor([[0, 1, 2]], dtype=torch.int32, device="cuda")
+k = torch.randn(1, 150, 2, 128, device="cuda").bfloat16()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    pc.write(p, table, 0, rope.apply(k, t), k)
+    pc.copy_pages(p, [0], [5])
+    outs = [pc.attend(k[:, :n].contiguous(), p, table, 150) for n in (1, 150)]
+    back = pc.window(p, table, 0, 150)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(outs[0], pc.attend(k[:, :1].contiguous(), p, table, 150))
+assert torch.equal(outs[1], pc.attend(k, p, table, 150)) and torch.equal(back[0], pc.window(p, table, 0, 150)[0])
+assert torch.equal(p.k[5], p.k[0]) and bool(p.k.any()) and _lib.device_status() == 0
+print("captured")
+"""
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lingbot-world-v2-realtime_b200")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, PYTHONPATH=root))
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 # ------------------------------------------------------------------------------------------------ the cache as used
 @FORMATS
 def test_sessions_prefill_decode_fork_evict_compact(fmt):
@@ -366,7 +450,7 @@ def test_sessions_prefill_decode_fork_evict_compact(fmt):
     def rand(b, n, h):
         return torch.randn(b, n, h, 128, generator=g).bfloat16().cuda()
 
-    def step(sessions, new, causal=True, passes=1):
+    def step(sessions, new, causal=True, passes=1, at=None):
         plan = c.plan(sessions, new)
         b, n = len(sessions), max(plan.new)
         for layer in range(layers):
@@ -374,7 +458,9 @@ def test_sessions_prefill_decode_fork_evict_compact(fmt):
                 k, v, q = rand(b, n, heads), rand(b, n, heads), rand(b, n, heads * group)
                 before = [x.cpu() for x in (c.layers[layer].k, c.layers[layer].v, c.layers[layer].k_amax, c.layers[layer].v_amax)]
                 rows = plan.start[:, None] + torch.arange(n, device="cuda")
-                c.write(layer, plan, k, v, rope=t)
+                if at is not None:
+                    rows = rows + i32([at.get(s, 0) for s in sessions])[:, None]
+                c.write(layer, plan, k, v, rope=t, positions=None if at is None else rows.contiguous())
                 kr = rope.apply(k, t, rows)
                 table = plan.table.cpu()
                 P.write(before[0], before[2], table, plan.held, plan.new, kr.cpu(), fmt)
@@ -402,16 +488,18 @@ def test_sessions_prefill_decode_fork_evict_compact(fmt):
     assert max(c.page_ids(a) + c.page_ids(f)) == c.num_pages - c.free_pages - 1
     for i in range(layers):
         assert torch.equal(raw(c.layers[i].k[c.page_ids(a)]), raw(kept[i]))
-    step([f, a], [1, 5])
+    with pytest.raises(ValueError, match="positions"):
+        step([f, a], [1, 5])
+    step([f, a], [1, 5], at={f: 64})                          # 64 tokens were evicted from f: positions follow on
     # a captured decode step: the plan's tensors take the next step's values
     plan = c.fixed_plan(2)
     k, v, q = rand(2, 1, heads), rand(2, 1, heads), rand(2, 1, heads * group)
     c.plan([a, f], 1, into=plan)
-    c.write(0, plan, k, v, rope=t)
+    c.write(0, plan, k, v)
     c.attend(0, plan, q)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        c.write(0, plan, k, v, rope=t)
+        c.write(0, plan, k, v)
         out = c.attend(0, plan, q, causal=True)
     for _ in range(3):
         for x, h in ((k, heads), (v, heads), (q, heads * group)):
