@@ -7,5 +7,7 @@ Public surface (mirrors the reference's modules of the same role):
                         that replaces lingbot/layers/sage_preq.py:attend
   split                 sequence split across GPUs (replaces lingbot/parallel/split_dit.py's
                         exchange and the head-divisibility rule of lingbot/parallel/config.py)
+  paged_cache           a KV cache that stays in 8 bits, in pages that sessions share, fork and drop
+  rope                  rotary tables and rotation
 """
-__all__ = ["attention", "kv_cache", "ops", "split"]
+__all__ = ["attention", "kv_cache", "ops", "paged_cache", "rope", "split"]
