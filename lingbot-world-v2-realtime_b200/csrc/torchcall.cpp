@@ -153,6 +153,31 @@ struct Pool {
         pages(integer(o, 4)), heads(int(integer(o, 5))), fmt(int(integer(o, 6))) {}
 };
 
+// pool(k, v, k_amax, v_amax): (device, heads, pool args or None where it has layers, page_copy's args)
+PyObject* pool(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) Py_RETURN_NONE;
+  const at::Tensor *k = tensor(args[0]), *v = tensor(args[1]), *ka = tensor(args[2]), *va = tensor(args[3]);
+  if (!k || !v || !ka || !va || !k->is_cuda()) Py_RETURN_NONE;
+  const auto type = k->scalar_type();
+  const int64_t d = k->dim();
+  if ((type != at::kChar && type != at::kFloat8_e4m3fn) || v->scalar_type() != type || ka->scalar_type() != at::kFloat ||
+      va->scalar_type() != at::kFloat || (d != 4 && d != 5) || k->size(d - 2) != 64 || k->size(d - 1) != 128 ||
+      v->sizes() != k->sizes() || ka->sizes() != k->sizes().slice(0, d - 2) || va->sizes() != ka->sizes() ||
+      !k->is_contiguous() || !v->is_contiguous() || !ka->is_contiguous() || !va->is_contiguous() ||
+      v->device() != k->device() || ka->device() != k->device() || va->device() != k->device())
+    Py_RETURN_NONE;
+  const long long pages = k->size(d - 4), heads = k->size(d - 3), layers = d == 5 ? k->size(0) : 1;
+  const auto kp = reinterpret_cast<long long>(k->const_data_ptr()), vp = reinterpret_cast<long long>(v->const_data_ptr());
+  const auto kap = reinterpret_cast<long long>(ka->const_data_ptr()), vap = reinterpret_cast<long long>(va->const_data_ptr());
+  const long long fmt = type == at::kChar ? 0 : 1;
+  PyObject* one = d == 5 ? Py_NewRef(Py_None) : Py_BuildValue("(LLLLLLL)", kp, kap, vp, vap, pages, heads, fmt);
+  if (one == nullptr) return nullptr;
+  return Py_BuildValue("(iLN(LLLLLLLLL))", int(k->get_device()), heads, one, kp, kap, vp, vap, pages, heads, layers,
+                       pages * heads * 64 * 128, pages * heads);
+  END_HANDLE_TH_ERRORS
+}
+
 // page_write(pool, device, table, start, k, v, lens or None, rope args or None, positions or None): 0
 PyObject* page_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -282,7 +307,7 @@ PyObject* page_copy(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(init), FAST(rope), FAST(page_write), FAST(page_read), FAST(page_copy), FAST(paged_attn),
+PyMethodDef methods[] = {FAST(init), FAST(pool), FAST(rope), FAST(page_write), FAST(page_read), FAST(page_copy), FAST(paged_attn),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torchcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

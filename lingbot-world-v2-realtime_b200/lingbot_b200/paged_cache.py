@@ -31,16 +31,18 @@ FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _ACT = {torch.bfloat16: 0, torch.float16: 1}
 
 
-@dataclass
 class Pages:
     """A pool of pages: k, v codes [pages, heads, 64, 128] (int8 or float8_e4m3fn) and k_amax, v_amax f32 [pages, heads],
     or the same with a leading dimension of layers. value = code * amax / 127 (int8) or / 448 (e4m3)."""
-    k: torch.Tensor
-    v: torch.Tensor
-    k_amax: torch.Tensor
-    v_amax: torch.Tensor
 
-    def __post_init__(self):
+    def __init__(self, k, v, k_amax, v_amax):
+        self.k, self.v, self.k_amax, self.v_amax = k, v, k_amax, v_amax
+        r = _lib.fast().pool(k, v, k_amax, v_amax)
+        if r is None:
+            self._refuse()
+        self._dev, self.heads, self._args, self._copy_args = r
+
+    def _refuse(self):
         k, v, ka, va = self.k, self.v, self.k_amax, self.v_amax
         if k.dtype not in FORMATS or v.dtype != k.dtype or ka.dtype != torch.float32 or va.dtype != torch.float32:
             raise TypeError("pages: int8 or float8_e4m3fn codes and float32 amax, got "
@@ -49,19 +51,13 @@ class Pages:
                 or ka.shape != k.shape[:-2] or va.shape != ka.shape:
             raise ValueError(f"pages: codes [(layers,) pages, heads, {PAGE}, {HEAD_DIM}] and amax [(layers,) pages, heads], "
                              f"got {tuple(k.shape)}, {tuple(v.shape)}, {tuple(ka.shape)}, {tuple(va.shape)}")
-        if not (k.is_contiguous() and v.is_contiguous() and ka.is_contiguous() and va.is_contiguous()):
-            raise ValueError("pages must be contiguous")
-        dev = k.device
-        if not k.is_cuda or v.device != dev or ka.device != dev or va.device != dev:
+        if not k.is_cuda or any(t.device != k.device for t in (v, ka, va)):
             raise ValueError("pages must be CUDA tensors of one device")
-        self.device = dev
-        self._dev = k.get_device()
-        self.heads = k.shape[-3]
-        layers, n = (k.shape[0] if k.dim() == 5 else 1), k.shape[-4] * self.heads
-        self._copy_args = (k.data_ptr(), ka.data_ptr(), v.data_ptr(), va.data_ptr(), k.shape[-4], self.heads, layers,
-                           n * PAGE * HEAD_DIM, n)
-        self._args = None if k.dim() == 5 else (k.data_ptr(), ka.data_ptr(), v.data_ptr(), va.data_ptr(), k.shape[0],
-                                                self.heads, FORMATS[k.dtype])
+        raise ValueError("pages must be contiguous")
+
+    @property
+    def device(self):
+        return self.k.device
 
     def layer(self, i) -> "Pages":
         """The pool of one layer."""
