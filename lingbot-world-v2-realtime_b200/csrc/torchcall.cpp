@@ -105,6 +105,24 @@ bool positions(PyObject* o, int dev, int64_t b, int64_t l, Positions* out) {
 }
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream(); }
 
+// rope_table(cos, sin, interleaved): (rotated channels, device, table args)
+PyObject* rope_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* c = n == 3 ? tensor(args[0]) : nullptr;
+  const at::Tensor* s = n == 3 ? tensor(args[1]) : nullptr;
+  if (!c || !s || c->scalar_type() != at::kFloat || s->scalar_type() != at::kFloat || !c->is_cuda() ||
+      c->device() != s->device() || c->dim() != 2 || c->sizes() != s->sizes() || c->strides() != s->strides() ||
+      c->stride(1) != 1)
+    Py_RETURN_NONE;
+  const int inter = PyObject_IsTrue(args[2]);
+  if (inter < 0) return nullptr;
+  const long long rot = 2 * c->size(1);
+  return Py_BuildValue("(Li(LLLLLi))", rot, int(c->get_device()), reinterpret_cast<long long>(c->const_data_ptr()),
+                       reinterpret_cast<long long>(s->const_data_ptr()), static_cast<long long>(c->stride(0)),
+                       static_cast<long long>(c->size(0)), rot, inter);
+  END_HANDLE_TH_ERRORS
+}
+
 // rope(x, k or None, table args, table device, positions or None, start, inverse)
 PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -307,7 +325,8 @@ PyObject* page_copy(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(init), FAST(pool), FAST(rope), FAST(page_write), FAST(page_read), FAST(page_copy), FAST(paged_attn),
+PyMethodDef methods[] = {FAST(init),      FAST(pool),      FAST(rope_table), FAST(rope),
+                         FAST(page_write), FAST(page_read), FAST(page_copy),  FAST(paged_attn),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torchcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

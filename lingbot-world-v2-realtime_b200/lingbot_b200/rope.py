@@ -7,8 +7,6 @@ tables here are fp32 rows by position, shared by any number of sessions and by `
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
-
 import torch
 
 from . import _lib
@@ -19,25 +17,23 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _POS = (torch.int32, torch.int64)
 
 
-@dataclass
 class Rope:
     """Rotary tables: cos, sin f32 [positions, rot / 2] on the GPU, rot the rotated channels of a head."""
-    cos: torch.Tensor
-    sin: torch.Tensor
-    interleaved: bool = True
 
-    def __post_init__(self):
+    def __init__(self, cos, sin, interleaved=True):
+        self.cos, self.sin, self.interleaved = cos, sin, interleaved
+        r = _lib.fast().rope_table(cos, sin, interleaved)
+        if r is None:
+            self._refuse()
+        self.rot, self._dev, self._args = r
+
+    def _refuse(self):
         c, s = self.cos, self.sin
         if not (c.dtype == s.dtype == torch.float32 and c.dim() == 2 and c.shape == s.shape and c.stride() == s.stride()
                 and c.stride(1) == 1 and c.device == s.device):
             raise ValueError("rope tables: two float32 [positions, rot / 2] tensors of one device and layout with unit "
                              f"last stride, got {c.dtype} {tuple(c.shape)} and {s.dtype} {tuple(s.shape)}")
-        if not c.is_cuda:
-            raise ValueError("rope tables must be CUDA tensors")
-        rows, half = c.shape
-        self.rot = 2 * half
-        self._dev = c.get_device()
-        self._args = (c.data_ptr(), s.data_ptr(), c.stride(0), rows, 2 * half, int(self.interleaved))
+        raise ValueError("rope tables must be CUDA tensors")
 
     def args(self, positions, device, b, l):
         """The table and position arguments of the C ABI, for tokens [b, l]."""

@@ -1,6 +1,10 @@
 """The paged 8-bit cache on the GPU against tests/_paged.py in float64: written codes and scales bit for bit, read-back
 values within the output's rounding, attention within the tolerance derived in _paged.attend plus half a step of the
 output type."""
+import bisect
+import math
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -89,6 +93,43 @@ def test_write_non_finite_huge_and_tiny(fmt):
         assert torch.equal(raw(x), raw(y))
     x, _ = pc.window(got, table.cuda(), 0, 20)
     assert bool(torch.isfinite(x).all())
+
+
+def exact_code(x, fmt):
+    """The code nearest to a fraction, half way cases to the even one."""
+    grid = [float(i) for i in range(128)] if fmt == torch.int8 else P.values(torch.arange(127, dtype=torch.uint8).view(fmt)).tolist()
+    hi = max(1, bisect.bisect_left(grid, abs(x)))
+    below, above = abs(x) - Fraction(grid[hi - 1]), Fraction(grid[hi]) - abs(x)
+    i = hi if above < below or (above == below and hi % 2 == 0) else hi - 1
+    return -grid[i] if x < 0 else grid[i]
+
+
+@FORMATS
+@TYPES
+def test_held_codes_half_way_between_two_go_to_the_even_one(fmt, dtype):
+    """Every code a page can hold, under growths of its scale by simple ratios, against rational arithmetic: c * old / a
+    is half way between two codes for many of them, whichever way old / a itself would be rounded in any precision."""
+    from lingbot_b200 import paged_cache as pc
+    ratios = [(n, d) for d in range(2, 24) for n in range(1, d) if math.gcd(n, d) == 1]
+    held = torch.arange(256, dtype=torch.uint8).view(torch.int8)
+    held = torch.where(held == -128, 0, held) if fmt == torch.int8 else torch.where((held & 127) == 127, 0, held).view(fmt)
+    held = P.to_codes(P.values(held), fmt)
+    n = len(ratios)
+    codes = torch.zeros(1, n, 64, 128, dtype=torch.int8).view(fmt)
+    codes.view(torch.int8)[0, :, :2] = held.view(torch.int8).reshape(2, 128)
+    amax = torch.tensor([[float(r[0]) for r in ratios]])
+    x = torch.zeros(1, 1, n, 128, dtype=dtype)
+    x[0, 0, :, 0] = torch.tensor([float(r[1]) for r in ratios])
+    got = pool((codes, codes.clone(), amax, amax.clone()))
+    pc.write(got, i32([[0]]), 2, x.cuda(), x.cuda())
+    ties = 0
+    for h, (old, a) in enumerate(ratios):
+        value = P.values(held).tolist()
+        want = [exact_code(Fraction(c) * old / a, fmt) for c in value]
+        ties += sum((Fraction(c) * old / a).denominator == 2 for c in value)
+        for pages in (got.k, got.v):
+            assert P.values(pages[0, h, :2].cpu()).flatten().tolist() == want, (old, a)
+    assert fmt != torch.int8 or ties > 1000
 
 
 @TYPES
