@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "../../include/lbq.h"
@@ -274,11 +275,17 @@ int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t ma
   const int64_t pages = (max_kv_len + lbq::kPageTokens - 1) / lbq::kPageTokens;
   // Few rows: two CTAs an SM (296 at once), a split keeps at least 4 pages, one for each warp. Many rows: one CTA an SM, at
   // least 8 pages to pay for the query tiles. Ragged batches get more and shorter splits, which balance the long sequences
-  // (measured, us: 256 CTAs of at most 8192 keys with 1 / 2 / 4 splits, all alike 84 / 93 / 100, lengths spread over 1..8192
-  // 79 / 65 / 61; 96 CTAs of at most 4100 keys with 3 / 4 / 6, ragged 25 / 22 / 19; with 3 / 4, all alike 27 / 34).
+  // (measured, us: CTAs before splitting x longest sequence, with 1 / 2 / 4 / 8 splits. 256 x 8192 keys, all alike 84 / 93 / 100;
+  // ragged 74 / 65 / 60 / 62; 512 x 8192 ragged 117 / 107 / 103; 1024 x 4096 ragged 98 / 104 / 113; 128 x 8192 ragged 51 / 41 /
+  // 28 / 32; 64 x 30000 ragged - / 91 / 70 / 48; 96 x 4100 with 3 / 4 / 6 splits, ragged 25 / 22 / 18, all alike 27 / 34). More
+  // CTAs than SMs want splits of 32 pages and more (ragged, 1 / 2 / 4: 192 x 2048 keys 23 / 20 / 22, 480 x 3000 45 / 48 / 49,
+  // 512 x 2048 35 / 39 / 44, 512 x 30000 366 / 330 / 312).
   const bool few = tile != lbq::kManyTile;
   int64_t n = (few ? kFewCtas : 148) / ctas;
-  if (few && ragged && pages >= 32 && ctas >= 64 && ctas <= 400) n = ctas <= 148 ? 2 * n : 2;
+  if (few && ragged && pages >= 32 && ctas >= 64 && ctas <= 600) {
+    if (ctas <= 148) n *= 2;
+    else n = std::max<int64_t>(std::min<int64_t>(4, pages / 32), ctas <= 400 ? 2 : 1);
+  }
   const int64_t least = few ? 4 : 8;
   if (n > pages / least) n = pages / least;
   if (few && n > 8 && n <= 16 && pages <= 96) n = 8;      // one cluster's worth: no merge launch (16 splits of 64 pages: alike)
