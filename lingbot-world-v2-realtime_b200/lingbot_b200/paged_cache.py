@@ -415,7 +415,7 @@ class PagedCache:
             total = (tokens + n + PAGE - 1) // PAGE
             if total > self.max_pages:
                 raise ValueError(f"session {s}: {tokens + n} tokens exceed {self.max_pages} pages")
-            need += total - len(pages)
+            need += max(0, total - len(pages))       # pages left from a larger plan that was not committed are no one else's
             if n and tokens % PAGE:
                 last = pages[tokens // PAGE]
                 left = refs.get(last, self._refs[last])

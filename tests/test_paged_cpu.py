@@ -247,3 +247,35 @@ def test_copy_pages_refuses_overlap():
         with pytest.raises(ValueError, match=word):
             paged_cache.copy_pages(None, src, dst)
     paged_cache.copy_pages(None, [], [])
+
+
+def _state(c):
+    return c.free_pages, list(c._refs), {s: (c.page_ids(s), c.tokens(s)) for s in c._sessions}
+
+
+def test_a_plan_that_does_not_fit_changes_nothing_beside_surplus_pages(monkeypatch):
+    """A session that still holds the pages of a larger plan, never committed, lends none of them to the others."""
+    pool = Tokens(monkeypatch, 8)
+    c = pool.cache
+    a, b = c.open(), c.open()
+    c.plan([a], 300)
+    before = _state(c)
+    with pytest.raises(RuntimeError, match="free"):
+        c.plan([a, b], [1, 400])
+    assert _state(c) == before
+    # the same with pages that are shared: the forks' unfinished page would have to be copied
+    pool = Tokens(monkeypatch, 7)
+    c = pool.cache
+    a, b = c.open(), c.open()
+    c.plan([a], 300)
+    plan = c.plan([b], 10)
+    pool.write(plan, [list(range(10))])
+    c.commit(plan)
+    d = c.fork(b)
+    c.fork(b)
+    before = _state(c)
+    with pytest.raises(RuntimeError, match="free"):
+        c.plan([a, b, d], 1)
+    assert _state(c) == before and pool.read(b) == pool.read(d) == list(range(10))
+    c.commit(c.plan([a, b], 1))                                     # what does fit
+    assert pool.read(b)[:10] == pool.read(d) == list(range(10)) and c.free_pages == 0
