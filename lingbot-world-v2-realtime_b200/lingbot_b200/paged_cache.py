@@ -426,15 +426,17 @@ class PagedCache:
         if need > len(self._free):
             raise RuntimeError(f"{need} pages needed, {len(self._free)} of {self.num_pages} free")
         if copies:
-            src, dst = [], []
-            for s, at in copies:
-                pages = self._sessions[s][0]
-                src.append(pages[at])
-                pages[at] = self._take()
-                dst.append(pages[at])
-                self._refs[src[-1]] -= 1
+            src, dst = [self._sessions[s][0][at] for s, at in copies], [self._take() for _ in copies]
+            try:
+                copy_pages(self.pages, src, dst)
+            except BaseException:
+                for p in dst:
+                    self._drop(p)
+                raise
+            for (s, at), old, new_page in zip(copies, src, dst):
+                self._sessions[s][0][at] = new_page
+                self._refs[old] -= 1
                 self._touch(s)
-            copy_pages(self.pages, src, dst)
         for s, n in zip(sessions, new):
             pages, tokens = self._sessions[s][:2]
             while len(pages) * PAGE < tokens + n:

@@ -279,3 +279,19 @@ def test_a_plan_that_does_not_fit_changes_nothing_beside_surplus_pages(monkeypat
     assert _state(c) == before and pool.read(b) == pool.read(d) == list(range(10))
     c.commit(c.plan([a, b], 1))                                     # what does fit
     assert pool.read(b)[:10] == pool.read(d) == list(range(10)) and c.free_pages == 0
+
+
+def test_a_copy_that_fails_leaves_the_sessions_as_they_were(monkeypatch):
+    pool = Tokens(monkeypatch, 8)
+    c = pool.cache
+    a = c.open()
+    c.commit(c.plan([a], 10))
+    c.fork(a)
+    before = _state(c)
+
+    def fails(pages, src, dst):
+        raise RuntimeError("no copy")
+    monkeypatch.setattr(paged_cache, "copy_pages", fails)
+    with pytest.raises(RuntimeError, match="no copy"):
+        c.plan([a], 1)
+    assert _state(c) == before
