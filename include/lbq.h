@@ -385,7 +385,7 @@ LBQ_API int lbq_rope(const void* x, int64_t sx_b, int64_t sx_l, int64_t sx_h, vo
                      int dtype, void* stream);
 
 /* Quantizing write of new tokens k, v [B, L, heads, 128] (dtype bf16 or fp16) at tokens start[b] .. start[b] + lens[b]
- * of each sequence (start null: start0 for all; lens null: L). For a page and head that new tokens x enter, a = max(amax
+ * of each sequence (start null: start0, below 2^62, for all; lens null: L). For a page and head that new tokens x enter, a = max(amax
  * of the tokens it holds before start, max finite |x|, 2^-40); its held codes become round(c * a_old / a), the new ones
  * round(x * Q / a) (exact decisions; int8 half to even, e4m3 to nearest); infinities become +-Q and NaN 0. Rows at and
  * past start that get no new token keep their codes. With rope tables (see lbq_rope; rot a multiple of 8, or of 16 for

@@ -15,6 +15,11 @@ namespace {
 using lbq::set_error;
 
 constexpr int kMaxGrid = 65535;
+constexpr int64_t kMaxStart = int64_t(1) << 62;      // a token index behind it could pass 64 bits
+
+int check_start(int64_t start) {
+  return start >= 0 && start < kMaxStart ? LBQ_OK : set_error(LBQ_ERR_ARG, "start must be >= 0 and below 2^62");
+}
 
 bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -122,7 +127,7 @@ int lbq_rope(const void* x, int64_t sx_b, int64_t sx_l, int64_t sx_h, void* y, i
   lbq::RopeArgs a{};
   if ((r = make_rope(&a.rope, rope_cos, rope_sin, rope_stride, rope_rows, rot, interleaved, pos, pos64, sp_b, sp_l, dim)))
     return r;
-  if (start < 0) return set_error(LBQ_ERR_ARG, "start must be >= 0");
+  if ((r = check_start(start))) return r;
   if (len == 0) return LBQ_OK;
   const int vec = 16 / size;
   // 16-byte accesses where a 16-byte piece lies wholly in the rotated part (or in one half of it) or in the rest
@@ -161,7 +166,7 @@ int lbq_page_write(const void* k, int64_t sk_b, int64_t sk_l, int64_t sk_h, cons
       (r = check_pool(k_pages, k_amax, v_pages, v_amax, num_pages, heads, fmt)) ||
       (r = check_batch(batch, len, "len")) || (r = check_table(table, st_b, width, batch)))
     return r;
-  if (start0 < 0) return set_error(LBQ_ERR_ARG, "start must be >= 0");
+  if ((r = check_start(start0))) return r;
   if (start == nullptr && lens == nullptr && start0 + len > int64_t(width) * lbq::kPageTokens)
     return set_error(LBQ_ERR_ARG, "tokens [%lld, %lld) outside the %d-page table", (long long)start0,
                      (long long)(start0 + len), width);
@@ -206,7 +211,7 @@ int lbq_page_read(const void* k_pages, const float* k_amax, const void* v_pages,
       (r = check_pool(k_pages, k_amax, v_pages, v_amax, num_pages, heads, fmt)) ||
       (r = check_batch(batch, len, "len")) || (r = check_table(table, st_b, width, batch)))
     return r;
-  if (start0 < 0) return set_error(LBQ_ERR_ARG, "start must be >= 0");
+  if ((r = check_start(start0))) return r;
   if (start == nullptr && lens == nullptr && start0 + len > int64_t(width) * lbq::kPageTokens)
     return set_error(LBQ_ERR_ARG, "tokens [%lld, %lld) outside the %d-page table", (long long)start0,
                      (long long)(start0 + len), width);

@@ -28,7 +28,7 @@ namespace lbq {
 // Page of block `blk` of sequence b, or -1 (recording the status) when the table or the pool has no such page.
 __device__ __forceinline__ int page_of(const PageTable& pt, int b, int64_t blk, int* status) {
   int id = -1;
-  if (blk < pt.width) id = pt.table[b * pt.st_b + blk];
+  if (uint64_t(blk) < uint64_t(pt.width)) id = pt.table[b * pt.st_b + blk];
   if (id < 0 || id >= pt.num_pages) {
     if (status) atomicCAS(status, 0, kDevBadPage);
     return -1;

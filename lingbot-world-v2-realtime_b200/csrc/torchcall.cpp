@@ -71,12 +71,12 @@ bool table_ok(const at::Tensor& t, int dev, int64_t batch) {
   return t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == batch && t.size(1) > 0 && t.is_cuda() &&
          t.get_device() == dev && (t.stride(1) == 1 || t.size(1) == 1);
 }
-// A Python int that fits 64 bits and is not negative.
+// A Python int that is not negative and below 2^62 (a count of tokens can be added to it).
 bool whole(PyObject* o, int64_t* v) {
   if (!PyLong_CheckExact(o)) return false;
   *v = PyLong_AsLongLong(o);
   if (*v == -1 && PyErr_Occurred()) PyErr_Clear();
-  return *v >= 0;
+  return *v >= 0 && *v < (int64_t(1) << 62);
 }
 // A count of every sequence: int32 [batch] tensor or a non-negative int.
 bool count(PyObject* o, int dev, int64_t batch, const int32_t** p, int64_t* v) {

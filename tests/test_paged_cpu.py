@@ -295,3 +295,19 @@ def test_a_copy_that_fails_leaves_the_sessions_as_they_were(monkeypatch):
     with pytest.raises(RuntimeError, match="no copy"):
         c.plan([a], 1)
     assert _state(c) == before
+
+
+def test_starts_near_the_end_of_64_bits_are_refused():
+    """start + length would pass 64 bits and come out negative, a page in front of the table. Refused on the host, with
+    lens (a device pointer, which the host does not read) as well as without."""
+    lib = _lib.load()
+    keep, p = _aligned()
+    for s0 in ((1 << 63) - 1, (1 << 63) - 8, 1 << 62):
+        for lens in (None, p):
+            assert lib.lbq_page_read(p, p, p, p, 4, 1, 0, p, 4, 4, None, s0, lens, 1, 8, p, 1024, 128, 128, p, 1024, 128, 128, 0,
+                                     None) == 1 and b"start" in lib.lbq_last_error()
+            assert lib.lbq_page_write(p, 1024, 128, 128, p, 1024, 128, 128, p, p, p, p, 4, 1, 0, p, 4, 4, None, s0, lens, 1, 8,
+                                      None, None, 0, 0, 0, 0, None, 0, 0, 0, 0, None) == 1 and b"start" in lib.lbq_last_error()
+        assert lib.lbq_rope(p, 512, 128, 128, p, 512, 128, 128, 1, None, 0, 0, 0, None, 0, 0, 0, 0, 1, 4, 128, p, p, 64, 4, 128, 1,
+                            None, 0, 0, 0, s0, 0, 0, None) == 1 and b"start" in lib.lbq_last_error()
+    del keep

@@ -551,3 +551,19 @@ def test_sessions_prefill_decode_fork_evict_compact(fmt):
         assert torch.allclose(out.float(), eager.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
         c.commit(plan)
         c.plan([a, f], 1, into=plan)
+
+
+# ------------------------------------------------------------------------------------------------ ends of the ranges
+def test_starts_that_pass_64_bits_are_refused():
+    from lingbot_b200 import paged_cache as pc, rope
+    p = pool(P.make_pages(8, 4, 2, torch.int8))
+    table, one = i32([[0, 1], [2, 3]]), i32([1, 1])
+    k = torch.randn(2, 3, 2, 128).bfloat16().cuda()
+    for s0 in (1 << 62, (1 << 63) - 1):
+        for lens in (None, one):
+            with pytest.raises(ValueError, match="64 bits"):
+                pc.window(p, table, s0, 3, lens=lens)
+            with pytest.raises(ValueError, match="64 bits"):
+                pc.write(p, table, s0, k, k, lens=lens)
+        with pytest.raises(ValueError, match="start"):
+            rope.apply(k, rope.tables(8, 64), start=s0)
