@@ -465,16 +465,20 @@ class PagedCache:
         return Plan([None] * batch, [0] * batch, [0] * batch,
                     torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=dev), z[0], z[1], z[2], [-1] * batch)
 
-    def _check(self, plan):
-        for s, v in zip(plan.sessions, plan.versions):
+    def _check(self, plan, committed=False):
+        """The plan still holds: its sessions' pages are those of the plan, and their tokens too (with `committed`, also with
+        the plan's own behind them)."""
+        for s, v, n, h in zip(plan.sessions, plan.versions, plan.new, plan.held):
             entry = self._sessions.get(s)
             if entry is None or entry[2] != v:
                 raise RuntimeError(f"session {s} was closed, forked, copied, evicted from or compacted since the plan was "
                                    "made: plan again")
+            if entry[1] != h and not (committed and entry[1] == h + n):
+                raise RuntimeError(f"session {s} moved on since the plan was made")
 
     def write(self, layer, plan: Plan, k, v, rope: Rope = None, positions=None):
         """Writes the plan's new tokens k, v [B, L, heads, 128] of one layer (L at least the longest session's new
-        tokens). Writing a plan again replaces them (the passes of one chunk)."""
+        tokens). Writing a plan again replaces them (the passes of one chunk), until it is committed."""
         self._check(plan)
         if k.dim() == 4 and k.shape[1] < max(plan.new):
             raise ValueError(f"{k.shape[1]} tokens given, {max(plan.new)} planned")
@@ -484,16 +488,13 @@ class PagedCache:
 
     def attend(self, layer, plan: Plan, q, causal=False, sm_scale=None, out=None, return_lse=False):
         """Attention of the plan's new tokens q [B, L, heads, 128] over everything their sessions hold."""
-        self._check(plan)
+        self._check(plan, committed=True)
         return attend(q, self.layers[layer], plan.table, plan.kv_lens, q_lens=plan.lens, causal=causal, sm_scale=sm_scale,
                       out=out, return_lse=return_lse)
 
     def commit(self, plan: Plan):
         """The plan's new tokens belong to their sessions from now on."""
         self._check(plan)
-        for s, n, h in zip(plan.sessions, plan.new, plan.held):
-            if self._get(s)[1] != h:
-                raise RuntimeError(f"session {s} moved on since the plan was made")
         for s, n in zip(plan.sessions, plan.new):
             self._sessions[s][1] += n
 

@@ -311,3 +311,33 @@ def test_starts_near_the_end_of_64_bits_are_refused():
         assert lib.lbq_rope(p, 512, 128, 128, p, 512, 128, 128, 1, None, 0, 0, 0, None, 0, 0, 0, 0, 1, 4, 128, p, p, 64, 4, 128, 1,
                             None, 0, 0, 0, s0, 0, 0, None) == 1 and b"start" in lib.lbq_last_error()
     del keep
+
+
+def test_a_plan_ends_when_its_session_goes_on(monkeypatch):
+    """After a commit the plan writes no more: its pages hold the tokens of later plans, whose scale a write would change.
+    It still attends until the next commit, to what was committed."""
+    pool = Tokens(monkeypatch, 12)
+    c = pool.cache
+    calls = []
+    monkeypatch.setattr(paged_cache, "write", lambda *a, **kw: calls.append("write"))
+    monkeypatch.setattr(paged_cache, "attend", lambda *a, **kw: calls.append("attend"))
+    a, b = c.open(), c.open()
+    x = torch.zeros(2, 10, 1, 128)
+    p1 = c.plan([a, b], [10, 0])
+    c.write(0, p1, x, x)
+    c.write(1, p1, x, x)
+    c.attend(0, p1, x)
+    c.commit(p1)
+    c.attend(1, p1, x)
+    assert calls == ["write", "write", "attend", "attend"]
+    with pytest.raises(RuntimeError, match="moved on"):
+        c.write(1, p1, x, x)
+    p2 = c.plan([a], 5)
+    c.write(0, p2, x, x)
+    with pytest.raises(RuntimeError, match="moved on"):
+        c.write(0, p1, x, x)
+    c.commit(p2)
+    for call in (lambda: c.write(0, p1, x, x), lambda: c.attend(0, p1, x), lambda: c.commit(p1), lambda: c.commit(p2)):
+        with pytest.raises(RuntimeError, match="moved on"):
+            call()
+    c.attend(0, p2, x)
