@@ -487,8 +487,11 @@ class PagedCache:
         write(self.layers[layer], plan.table, plan.start, k, v, lens=plan.lens, rope=rope, positions=positions)
 
     def attend(self, layer, plan: Plan, q, causal=False, sm_scale=None, out=None, return_lse=False):
-        """Attention of the plan's new tokens q [B, L, heads, 128] over everything their sessions hold."""
+        """Attention of the plan's new tokens q [B, L, heads, 128] (L at least the longest session's new tokens) over
+        everything their sessions hold."""
         self._check(plan, committed=True)
+        if q.dim() == 4 and q.shape[1] < max(plan.new):              # the rows there are would count as the last tokens
+            raise ValueError(f"{q.shape[1]} queries given, {max(plan.new)} tokens planned")
         return attend(q, self.layers[layer], plan.table, plan.kv_lens, q_lens=plan.lens, causal=causal, sm_scale=sm_scale,
                       out=out, return_lse=return_lse)
 

@@ -341,3 +341,16 @@ def test_a_plan_ends_when_its_session_goes_on(monkeypatch):
         with pytest.raises(RuntimeError, match="moved on"):
             call()
     c.attend(0, p2, x)
+
+
+def test_attend_wants_a_query_for_every_planned_token(monkeypatch):
+    """Fewer rows would be taken for the sequence's last tokens, under a causal mask that is shifted."""
+    pool = Tokens(monkeypatch, 12)
+    c = pool.cache
+    monkeypatch.setattr(paged_cache, "attend", lambda q, *a, **kw: q.shape[1])
+    a, b = c.open(), c.open()
+    plan = c.plan([a, b], [90, 3])
+    for n in (0, 60, 89):
+        with pytest.raises(ValueError, match="90 tokens"):
+            c.attend(0, plan, torch.zeros(2, n, 1, 128), causal=True)
+    assert c.attend(0, plan, torch.zeros(2, 90, 1, 128)) == 90 and c.attend(0, plan, torch.zeros(2, 128, 1, 128)) == 128
