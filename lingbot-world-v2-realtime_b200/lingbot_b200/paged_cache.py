@@ -484,6 +484,10 @@ class PagedCache:
             raise ValueError(f"{k.shape[1]} tokens given, {max(plan.new)} planned")
         if rope is not None and positions is None and any(self._sessions[s][3] for s in plan.sessions):
             raise ValueError("tokens were evicted from a session of this plan: pass the new tokens' positions")
+        if rope is not None and positions is None:
+            last = max((h + n for h, n in zip(plan.held, plan.new) if n), default=0)
+            if last > rope.cos.shape[0]:                             # their K would be stored as it is
+                raise ValueError(f"tokens up to {last} planned, rope tables of {rope.cos.shape[0]} positions")
         write(self.layers[layer], plan.table, plan.start, k, v, lens=plan.lens, rope=rope, positions=positions)
 
     def attend(self, layer, plan: Plan, q, causal=False, sm_scale=None, out=None, return_lse=False):
