@@ -359,17 +359,18 @@ def test_attend_wants_a_query_for_every_planned_token(monkeypatch):
 def test_write_refuses_rope_tables_that_end_before_the_tokens(monkeypatch):
     pool = Tokens(monkeypatch, 12)
     c = pool.cache
-    monkeypatch.setattr(paged_cache, "write", lambda *a, rope=None, **kw: rope)
+    written = []
+    monkeypatch.setattr(paged_cache, "write", lambda *a, rope=None, **kw: written.append(rope))
     r = type("R", (), {})()
     r.cos = torch.zeros(100, 64)
     a, b = c.open(), c.open()
     c.commit(c.plan([a], 100))
     k = torch.zeros(2, 101, 1, 128)
-    plan = c.plan([a, b], [0, 100])                                   # a writes nothing
-    assert c.write(0, plan, k, k, rope=r) is r
+    c.write(0, c.plan([a, b], [0, 100]), k, k, rope=r)                # a writes nothing
     for new in ([1, 5], [0, 101]):
         plan = c.plan([a, b], new)
         with pytest.raises(ValueError, match="100 positions"):
             c.write(0, plan, k, k, rope=r)
-        assert c.write(0, plan, k, k, rope=r, positions=torch.zeros(2, 101, dtype=torch.int32)) is r
-        assert c.write(0, plan, k, k) is None
+        c.write(0, plan, k, k, rope=r, positions=torch.zeros(2, 101, dtype=torch.int32))
+        c.write(0, plan, k, k)
+    assert written == [r, r, None, r, None]
