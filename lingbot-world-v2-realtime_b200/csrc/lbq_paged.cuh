@@ -19,6 +19,11 @@ __device__ __forceinline__ void after_previous_grid() {
 }
 
 constexpr float kTinyScale = 5.421010862427522e-20f;   // 2^-64: scales are kept above it (a written page's are >= 2^-40)
+constexpr float kMinFactor = 1.1754943508222875e-38f;  // 2^-126
+// The factor of a row's scores of one page, from the page's scale * softmax scale * log2 e / Q and the power of two taken out
+// of the row. In this order no product below it loses bits before the last; and it never is 0, which times the -inf of a
+// masked score would be NaN (scores stay below 2^17 in magnitude: at the smallest factor they are 0 to any precision).
+__device__ __forceinline__ float score_factor(float page, float row) { return fmaxf(page * row, kMinFactor); }
 constexpr float kWeightBits = 7.f;               // weights are scaled by 2^7 ...
 constexpr float kSlack = 8.f;                    // ... and the running maximum may lag by 2^8: below 2^15, fp16's range
 

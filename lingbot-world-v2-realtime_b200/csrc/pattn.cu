@@ -197,14 +197,14 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
   }
 
   uint2 qb[kNT][8];
-  float unit[kNT][2];                                    // per query column: undo the power of two, softmax scale, 1 / Q
+  float unit[kNT][2];                                    // per query column: the power of two taken out
   int limit[kNT][2];                                     // last visible key of the split (a table has under 2^24 pages)
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
     const int r = tile * kRows + 8 * t + r0, i = r / a.group, g = r - i * a.group;
     const uint16_t* row = i < tk.qn ? static_cast<const uint16_t*>(a.q) + b * a.sq[0] + i * a.sq[1] + (h * a.group + g) * a.sq[2]
                                     : nullptr;
-    const float u = load_query<kDt>(row, quad, qb[t]) * a.score_log2;
+    const float u = load_query<kDt>(row, quad, qb[t]);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       unit[t][e] = __shfl_sync(0xffffffffu, u, 8 * quad + 4 * e);      // column 2 quad + e is row r0 of that lane
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         }
     }
     const float kat = fmaxf(ka, kTinyScale), vat = fmaxf(va, kTinyScale);
-    const float lv = __log2f(vat), iv = __frcp_rn(vat);
+    const float ks = kat * a.score_log2, lv = __log2f(vat), iv = __frcp_rn(vat);
     const int j0 = i * kPageTokens;
     uint32_t pb[kNT][4][2];
 #pragma unroll
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         for (int mt = 1; mt < 4; ++mt) top = fmax3(top, x[t][mt][e], x[t][mt][2 + e]);
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        c[e] = kat * unit[t][e];
+        c[e] = score_factor(ks, unit[t][e]);
         top = fmaf(top, c[e], lv);
         al[e] = 1.f;
         if (top > m[t][e] + kSlack) {                    // also from m = -inf

@@ -278,13 +278,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
     const int row = tile * kManyTile + t * 128 + rl, qi = row / a.group, head = h * a.group + (row - qi * a.group);
     const bool on = qi < tk.qn;
     const uint16_t* qrow = on ? static_cast<const uint16_t*>(a.q) + b * a.sq[0] + qi * a.sq[1] + head * a.sq[2] : nullptr;
-    const float unit = stage_query<kDt>(qrow, sQ + t * kQTile, rl) * a.score_log2;
+    const float unit = stage_query<kDt>(qrow, sQ + t * kQTile, rl);
     fence_proxy_async_smem();
     mbar_arrive(&sh->q_full);
     const int limit = !on ? -1 : int((a.causal ? tk.kv - tk.qn + qi : tk.kv - 1) - int64_t(p0) * kPageTokens);
     float m = -INFINITY, l = 0.f;
     // The scales of the next page are loaded one page ahead, its id two pages ahead. They are kept above 0 (a written
-    // page's are at least 2^-40): a masked score is -inf times ka, and va is divided by.
+    // page's are at least 2^-40): the sum is divided by va, and its logarithm taken.
     int id_next = n > 0 ? table[0] : 0;
     float ka_next = 1.f, va_next = 1.f;
     bool ok_next = false;
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
 #pragma unroll
         for (int q = 0; q < 4; ++q) r[q] = fmax3(r[q], F(i + 2 * q), F(i + 2 * q + 1));
       }
-      const float c = ka * unit, lv = __log2f(va);
+      const float c = score_factor(ka * a.score_log2, unit), lv = __log2f(va);
       const float top = fmaf(fmax3(r[0], r[1], fmaxf(r[2], r[3])), c, lv);
       const bool grow = top > m + kSlack;                 // also from m = -inf
       if (__any_sync(0xffffffffu, grow)) {

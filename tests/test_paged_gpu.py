@@ -567,3 +567,22 @@ def test_starts_that_pass_64_bits_are_refused():
                 pc.write(p, table, s0, k, k, lens=lens)
         with pytest.raises(ValueError, match="start"):
             rope.apply(k, rope.tables(8, 64), start=s0)
+
+
+@FORMATS
+@pytest.mark.parametrize("lq", [4, 140], ids=["few", "many"])
+def test_attend_tiny_rows_on_pages_of_zeros(fmt, lq):
+    """Masked keys in pages whose K are zero (amax 2^-40, as a write leaves it, or 0) under query rows down to bf16's smallest
+    normal: the scores are 0 and no row becomes NaN. Scores of magnitude 1 from such rows and a page of 2^120 are right."""
+    k, v, ka, va = P.make_pages(13, 5, 1, fmt)
+    k.view(torch.int8)[1:4] = 0
+    ka[1:4] = torch.tensor([[2.0 ** -40], [2.0 ** -40], [0.0]])
+    ka[4] = 1.9 * 2.0 ** 120
+    table = torch.tensor([[0, 1, 2, 3], [4, 1, 3, -1]], dtype=torch.int32)
+    q = torch.randn(2, lq, 2, 128, generator=torch.Generator().manual_seed(3)) * 2.0 ** -118
+    q[0, ::4] *= 2.0 ** 118
+    q[0, 1::4] *= 2.0 ** 20
+    q[:, 3::4] = torch.where(q[:, 3::4] > 0, 2.0 ** -126, 0.0)
+    assert bool((q.bfloat16().abs().amax(-1) > 0).all())
+    for causal in (True, False):
+        run_attend(q.bfloat16(), (k, v, ka, va), table, [250, 190], [lq, lq], causal)
