@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
 #pragma unroll
         for (int q = 0; q < 4; ++q) r[q] = fmax3(r[q], F(i + 2 * q), F(i + 2 * q + 1));
       }
-      const float c = score_factor(ka * a.score_log2, unit), lv = __log2f(va);
+      const float c = score_factor(ka * a.score_log2, unit), lv = __log2f(va), iv = __frcp_rn(va);
       const float top = fmaf(fmax3(r[0], r[1], fmaxf(r[2], r[3])), c, lv);
       const bool grow = top > m + kSlack;                 // also from m = -inf
       if (__any_sync(0xffffffffu, grow)) {
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
       float s[4];
       f2_unpack(acc[0], s[0], s[1]);
       f2_unpack(acc[1], s[2], s[3]);
-      l += __fdividef((s[0] + s[1]) + (s[2] + s[3]), va);
+      l = fmaf((s[0] + s[1]) + (s[2] + s[3]), iv, l);     // (a quotient by __fdividef is 0 for va above 2^126)
     }
     if (ok && n > 0) ok = mbar_wait(&sh->o_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, a.status, kDevTimeoutO);
     tc_fence_after();

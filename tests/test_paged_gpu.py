@@ -586,3 +586,16 @@ def test_attend_tiny_rows_on_pages_of_zeros(fmt, lq):
     assert bool((q.bfloat16().abs().amax(-1) > 0).all())
     for causal in (True, False):
         run_attend(q.bfloat16(), (k, v, ka, va), table, [250, 190], [lq, lq], causal)
+
+
+@FORMATS
+@pytest.mark.parametrize("lq", [1, 129], ids=["few", "many"])
+def test_attend_values_up_to_the_largest(fmt, lq):
+    """V scales from 2^125 to bf16's largest finite value, which the write stores: in every page, and in some."""
+    k, v, ka, va = P.make_pages(15, 6, 1, fmt)
+    table = P.make_table(2, [5], 6)
+    q = torch.randn(1, lq, 2, 128, generator=torch.Generator().manual_seed(4)).bfloat16()
+    for scales in ([1.5 * 2.0 ** 126] * 6, [2.0 ** 125, 3.3895e38, 1.1 * 2.0 ** 126, 2.0 ** 127, 2.0 ** 120, 2.0 ** 126]):
+        va = torch.tensor(scales).bfloat16().float()[:, None]
+        for splits in (1, 3):
+            run_attend(q, (k, v, ka, va), table, [300], [lq], False, num_splits=splits)
