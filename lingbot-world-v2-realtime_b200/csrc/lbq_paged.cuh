@@ -20,10 +20,22 @@ __device__ __forceinline__ void after_previous_grid() {
 
 constexpr float kTinyScale = 5.421010862427522e-20f;   // 2^-64: scales are kept above it (a written page's are >= 2^-40)
 constexpr float kMinFactor = 1.1754943508222875e-38f;  // 2^-126
-// The factor of a row's scores of one page, from the page's scale * softmax scale * log2 e / Q and the power of two taken out
-// of the row. In this order no product below it loses bits before the last; and it never is 0, which times the -inf of a
-// masked score would be NaN (scores stay below 2^17 in magnitude: at the smallest factor they are 0 to any precision).
-__device__ __forceinline__ float score_factor(float page, float row) { return fmaxf(page * row, kMinFactor); }
+// The factor of a row's scores of one page: the page's scale, the power of two taken out of the row, and softmax scale *
+// log2 e / Q, which takes the larger of the two first: what underflows then is smaller still at the end. It never is 0,
+// which times the -inf of a masked score would be NaN (scores stay below 2^17 in magnitude: at the smallest factor they are 0
+// to any precision).
+__device__ __forceinline__ float score_factor(float page, float row, float scale) {
+  return fmaxf(fmaxf(page, row) * scale * fminf(page, row), kMinFactor);
+}
+// The power of two that scales a bf16 query row of largest magnitude `top` (the bits of the fp32 value) to a maximum in
+// [1, 2), and its inverse `up`. With the exponent field e that is 2^(127 - e); 2^(127 - 254) is no normal float: a maximum
+// in [2, 4) there. A row of subnormals, 2^-126 at most, goes up by 2^127; non-finite rows go as they are.
+__device__ __forceinline__ float row_scale(uint32_t top, float& up) {
+  const uint32_t e = min(top >> 23, 253u);
+  const bool finite = top < 0x7f800000u;
+  up = !finite ? 1.f : e == 0 ? 5.877471754111438e-39f : __uint_as_float(e << 23);      // 2^-127
+  return finite ? __uint_as_float((254u - e) << 23) : 1.f;
+}
 constexpr float kWeightBits = 7.f;               // weights are scaled by 2^7 ...
 constexpr float kSlack = 8.f;                    // ... and the running maximum may lag by 2^8: below 2^15, fp16's range
 

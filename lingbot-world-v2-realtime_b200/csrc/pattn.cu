@@ -82,12 +82,8 @@ __device__ __forceinline__ float load_query(const uint16_t* row, int quad, uint2
   } else {
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // exponent field e of the maximum: scale by 2^(127 - e); zero, subnormal and non-finite rows go unscaled
-    uint32_t e = top >> 23;
-    const bool plain = e == 0 || e == 255;
-    if (e == 254) e = 253;                               // 2^(127 - 254) is no normal float: a maximum in [2, 4)
-    const float down = plain ? 1.f : __uint_as_float((254u - e) << 23);
-    const float up = plain ? 1.f : __uint_as_float(e << 23);
+    float up;
+    const float down = row_scale(top, up);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const __half2 lo = __floats2half2_rn(__uint_as_float(raw[k].x << 16) * down, __uint_as_float(raw[k].x & 0xffff0000u) * down);
@@ -273,7 +269,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         }
     }
     const float kat = fmaxf(ka, kTinyScale), vat = fmaxf(va, kTinyScale);
-    const float ks = kat * a.score_log2, lv = __log2f(vat), iv = __frcp_rn(vat);
+    const float lv = __log2f(vat), iv = __frcp_rn(vat);
     const int j0 = i * kPageTokens;
     uint32_t pb[kNT][4][2];
 #pragma unroll
@@ -296,7 +292,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         for (int mt = 1; mt < 4; ++mt) top = fmax3(top, x[t][mt][e], x[t][mt][2 + e]);
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        c[e] = score_factor(ks, unit[t][e]);
+        c[e] = score_factor(kat, unit[t][e], a.score_log2);
         top = fmaf(top, c[e], lv);
         al[e] = 1.f;
         if (top > m[t][e] + kSlack) {                    // also from m = -inf

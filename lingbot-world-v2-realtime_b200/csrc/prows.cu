@@ -79,13 +79,7 @@ __device__ __forceinline__ float stage_query(const uint16_t* row, uint8_t* tile,
         for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
       }
     }
-    uint32_t e = top >> 23;
-    const bool plain = e == 0 || e == 255;
-    if (e == 254) e = 253;
-    if (!plain) {
-      down = __uint_as_float((254u - e) << 23);
-      up = __uint_as_float(e << 23);
-    }
+    down = row_scale(top, up);
   }
 #pragma unroll 4
   for (int c = 0; c < 16; ++c) {
@@ -327,7 +321,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
 #pragma unroll
         for (int q = 0; q < 4; ++q) r[q] = fmax3(r[q], F(i + 2 * q), F(i + 2 * q + 1));
       }
-      const float c = score_factor(ka * a.score_log2, unit), lv = __log2f(va), iv = __frcp_rn(va);
+      const float c = score_factor(ka, unit, a.score_log2), lv = __log2f(va), iv = __frcp_rn(va);
       const float top = fmaf(fmax3(r[0], r[1], fmaxf(r[2], r[3])), c, lv);
       const bool grow = top > m + kSlack;                 // also from m = -inf
       if (__any_sync(0xffffffffu, grow)) {

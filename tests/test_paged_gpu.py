@@ -599,3 +599,24 @@ def test_attend_values_up_to_the_largest(fmt, lq):
         va = torch.tensor(scales).bfloat16().float()[:, None]
         for splits in (1, 3):
             run_attend(q, (k, v, ka, va), table, [300], [lq], False, num_splits=splits)
+
+
+@FORMATS
+@pytest.mark.parametrize("lq", [2, 130], ids=["few", "many"])
+def test_attend_subnormal_rows(fmt, lq):
+    """bf16 query rows below its smallest normal, down to one smallest subnormal, and rows of zeros, against K so large that
+    the scores matter; the largest finite rows against K so small."""
+    k, v, ka, va = P.make_pages(16, 6, 1, fmt)
+    table = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32)
+    ka = torch.tensor([1.9 * 2.0 ** 126] * 3 + [2.0 ** -40] * 3).bfloat16().float()[:, None]
+    q = torch.randn(2, lq, 2, 128, generator=torch.Generator().manual_seed(5)).clamp(-3.9, 3.9)
+    q[0] = q[0] * 2.0 ** -129
+    q[0, 1::3] = 0
+    q[0, 1::3, 0, 17] = 2.0 ** -133
+    q[0, 1::3, 1] = 0
+    q[1] = q[1] / 4 * 3.3e38
+    q = q.bfloat16()
+    assert bool((q[0].float().abs() < 2.0 ** -126).all()) and bool(torch.isfinite(q).all()) and bool(q[0, 0].any())
+    for causal in (False, True):
+        run_attend(q[:1], (k, v, ka, va), table[:1], [150], [lq], causal)
+        run_attend(q[1:], (k, v, ka, va), table[1:], [190], [lq], causal, sm_scale=2.0 ** -85)
