@@ -20,13 +20,20 @@ __device__ __forceinline__ void after_previous_grid() {
 
 constexpr float kTinyScale = 5.421010862427522e-20f;   // 2^-64: scales are kept above it (a written page's are >= 2^-40)
 constexpr float kMinFactor = 1.1754943508222875e-38f;  // 2^-126
-// The factor of a row's scores of one page: the page's scale, the power of two taken out of the row, and softmax scale *
-// log2 e / Q, which takes the larger of the two first: what underflows then is smaller still at the end. It never is 0,
-// which times the -inf of a masked score would be NaN (scores stay below 2^17 in magnitude: at the smallest factor they are 0
-// to any precision).
-__device__ __forceinline__ float score_factor(float page, float row, float scale) {
-  return fmaxf(fmaxf(page, row) * scale * fminf(page, row), kMinFactor);
-}
+// The factor of a row's scores of one page: page (its scale) * row (the power of two taken out of the row) * scale (softmax
+// scale * log2 e / Q). Row and scale are multiplied first, raised by 2^64 where they would underflow though a large page
+// brings them back. It never is 0, which times the -inf of a masked score would be NaN (scores stay below 2^17 in magnitude:
+// at the smallest factor they are 0 to any precision).
+struct RowFactor {
+  float unit, lower;
+  __device__ __forceinline__ RowFactor() {}
+  __device__ __forceinline__ RowFactor(float row, float scale) {
+    const bool small = row * scale < 7.888609052210118e-31f;             // 2^-100
+    unit = small ? row * 18446744073709551616.f * scale : row * scale;
+    lower = small ? 5.421010862427522e-20f : 1.f;
+  }
+  __device__ __forceinline__ float of(float page) const { return fmaxf(page * unit * lower, kMinFactor); }
+};
 // The power of two that scales a bf16 query row of largest magnitude `top` (the bits of the fp32 value) to a maximum in
 // [1, 2), and its inverse `up`. With the exponent field e that is 2^(127 - e); 2^(127 - 254) is no normal float: a maximum
 // in [2, 4) there. A row of subnormals, 2^-126 at most, goes up by 2^127; non-finite rows go as they are.
@@ -38,6 +45,17 @@ __device__ __forceinline__ float row_scale(uint32_t top, float& up) {
 }
 constexpr float kWeightBits = 7.f;               // weights are scaled by 2^7 ...
 constexpr float kSlack = 8.f;                    // ... and the running maximum may lag by 2^8: below 2^15, fp16's range
+
+// A page whose largest weight lies more than 2^kFaint below 2^kWeightBits adds nothing to o, but may hold most of the sum
+// when its V are that much smaller (weights carry the scale of V, a page of zeros has 2^-40): its weights would underflow
+// before the division by va. The binary exponent that they, and va, are raised by; `top` is the page's and m the row's
+// maximum. (400: the page's part of the sum is 0 then, and masked pages, top = -inf, stay finite.) While sums are taken they
+// are scaled by 2^kSumBits, so that 1 / va (2^128 at most) is no subnormal.
+constexpr float kFaint = 100.f;
+constexpr float kSumBits = 8.f, kSumUnit = 1.f / 256.f;
+__device__ __forceinline__ float faint_exponent(float top, float m) { return fminf(fmaxf(m - top - kFaint, 0.f), 400.f); }
+// 2^(e / 2): l times it twice. 2^e alone can underflow where the maximum moves for a V scale and not for a score.
+__device__ __forceinline__ float half_ex2(float e) { return ex2_approx(0.5f * e); }
 
 // Keys [0, visible) are seen by some row of the tile; 0 when every row is empty or past the sequence's queries.
 struct TileKeys {

@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
   }
 
   uint2 qb[kNT][8];
-  float unit[kNT][2];                                    // per query column: the power of two taken out
+  RowFactor unit[kNT][2];                                // per query column
   int limit[kNT][2];                                     // last visible key of the split (a table has under 2^24 pages)
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
     const float u = load_query<kDt>(row, quad, qb[t]);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      unit[t][e] = __shfl_sync(0xffffffffu, u, 8 * quad + 4 * e);      // column 2 quad + e is row r0 of that lane
+      unit[t][e] = RowFactor(__shfl_sync(0xffffffffu, u, 8 * quad + 4 * e), a.score_log2);      // column 2 quad + e is row r0 of that lane
       const int qi = (tile * kRows + 8 * t + 2 * quad + e) / a.group;
       limit[t][e] = qi >= tk.qn ? -1 : int((a.causal ? tk.kv - tk.qn + qi : tk.kv - 1) - int64_t(p0) * kPageTokens);
     }
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         }
     }
     const float kat = fmaxf(ka, kTinyScale), vat = fmaxf(va, kTinyScale);
-    const float lv = __log2f(vat), iv = __frcp_rn(vat);
+    const float lv = __log2f(vat);
     const int j0 = i * kPageTokens;
     uint32_t pb[kNT][4][2];
 #pragma unroll
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
             if (!ok || j > limit[t][e & 1]) x[t][mt][e] = -INFINITY;
           }
       }
-      float c[2], bb[2], al[2];
+      float c[2], bb[2], half[2], is[2];
       bool grow = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -292,24 +292,29 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         for (int mt = 1; mt < 4; ++mt) top = fmax3(top, x[t][mt][e], x[t][mt][2 + e]);
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        c[e] = score_factor(kat, unit[t][e], a.score_log2);
+        c[e] = unit[t][e].of(kat);
         top = fmaf(top, c[e], lv);
-        al[e] = 1.f;
+        half[e] = 1.f;
         if (top > m[t][e] + kSlack) {                    // also from m = -inf
-          al[e] = ex2_approx(m[t][e] - top);
+          half[e] = half_ex2(m[t][e] - top);
           m[t][e] = top;
           grow = true;
         }
+        const float lift = lv + faint_exponent(top, m[t][e]);
+        is[e] = ex2_approx(kSumBits - lift);
         // a query that has seen no key yet: its exponents are taken against 0 and are -inf
-        bb[e] = lv - ((m[t][e] == -INFINITY ? 0.f : m[t][e]) - kWeightBits);
+        bb[e] = lift - ((m[t][e] == -INFINITY ? 0.f : m[t][e]) - kWeightBits);
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) l[t][e] *= al[e];
+        for (int e = 0; e < 2; ++e) {
+          l[t][e] = l[t][e] * half[e] * half[e];
+          half[e] *= half[e];
+        }
 #pragma unroll
         for (int c8 = 0; c8 < 8; ++c8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[c8][t][e] *= al[e & 1];
+          for (int e = 0; e < 4; ++e) o[c8][t][e] *= half[e & 1];
       }
       float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         pb[t][mt][1] = movmatrix_t(pack_act2(w[2], w[3], 1));
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) l[t][e] = fmaf(sum[e], iv, l[t][e]);
+      for (int e = 0; e < 2; ++e) l[t][e] = fmaf(sum[e], is[e], l[t][e]);
     }
     // rows of V past the sequence's tokens hold whatever the page held before: weight 0 times a NaN code (e4m3; int8 has
     // none) would be NaN, so they are read as 0
@@ -387,7 +392,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
       const int q = 8 * t + 2 * quad + e;
       if (r0 == 0) {
         sh.m[warp][q] = m[t][e];
-        sh.l[warp][q] = l[t][e];
+        sh.l[warp][q] = l[t][e] * kSumUnit;
       }
       float* row = mo + (warp * kRows + q) * kMergePitch + 2 * r0;
 #pragma unroll
@@ -408,8 +413,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
     for (int k = 0; k < 8; ++k) acc[k] = 0.f;
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
-      const float f = ex2_approx(sh.m[w][rr] - ref);
-      ll += sh.l[w][rr] * f;
+      const float half = half_ex2(sh.m[w][rr] - ref), f = half * half;
+      ll += sh.l[w][rr] * half * half;
       const float4* p = reinterpret_cast<const float4*>(mo + (w * kRows + rr) * kMergePitch + 8 * seg);
       const float4 x = p[0], y = p[1];
       acc[0] += x.x * f;
@@ -470,8 +475,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
     float2 o2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      const float f = ex2_approx(ml[s].x - ref);
-      ll += ml[s].y * f;
+      const float half = half_ex2(ml[s].x - ref), f = half * half;
+      ll += ml[s].y * half * half;
       o2.x += x[s].x * f;
       o2.y += x[s].y * f;
     }
@@ -521,14 +526,14 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs 
     float top = m;
 #pragma unroll
     for (int k = 0; k < kRound; ++k) top = fmaxf(top, ml[k].x);
-    const float ref = top == -INFINITY ? 0.f : top, al = ex2_approx(m - ref);
+    const float ref = top == -INFINITY ? 0.f : top, half = half_ex2(m - ref), al = half * half;
     m = top;
-    l *= al;
+    l = l * half * half;
     o = make_float4(o.x * al, o.y * al, o.z * al, o.w * al);
 #pragma unroll
     for (int k = 0; k < kRound; ++k) {
-      const float f = ex2_approx(ml[k].x - ref);
-      l += ml[k].y * f;
+      const float half_k = half_ex2(ml[k].x - ref), f = half_k * half_k;
+      l += ml[k].y * half_k * half_k;
       o.x += x[k].x * f;
       o.y += x[k].y * f;
       o.z += x[k].z * f;
@@ -547,9 +552,9 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs 
   o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const float f = ex2_approx(sm[w] - ref);
+    const float half = half_ex2(sm[w] - ref), f = half * half;
     const float4 x = so[w][lane];
-    l += sl[w] * f;
+    l += sl[w] * half * half;
     o.x += x.x * f;
     o.y += x.y * f;
     o.z += x.z * f;

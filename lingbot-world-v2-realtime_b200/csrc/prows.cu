@@ -272,13 +272,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
     const int row = tile * kManyTile + t * 128 + rl, qi = row / a.group, head = h * a.group + (row - qi * a.group);
     const bool on = qi < tk.qn;
     const uint16_t* qrow = on ? static_cast<const uint16_t*>(a.q) + b * a.sq[0] + qi * a.sq[1] + head * a.sq[2] : nullptr;
-    const float unit = stage_query<kDt>(qrow, sQ + t * kQTile, rl);
+    const RowFactor unit(stage_query<kDt>(qrow, sQ + t * kQTile, rl), a.score_log2);
     fence_proxy_async_smem();
     mbar_arrive(&sh->q_full);
     const int limit = !on ? -1 : int((a.causal ? tk.kv - tk.qn + qi : tk.kv - 1) - int64_t(p0) * kPageTokens);
     float m = -INFINITY, l = 0.f;
     // The scales of the next page are loaded one page ahead, its id two pages ahead. They are kept above 0 (a written
-    // page's are at least 2^-40): the sum is divided by va, and its logarithm taken.
+    // page's are at least 2^-40): the logarithm of va is taken.
     int id_next = n > 0 ? table[0] : 0;
     float ka_next = 1.f, va_next = 1.f;
     bool ok_next = false;
@@ -321,13 +321,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
 #pragma unroll
         for (int q = 0; q < 4; ++q) r[q] = fmax3(r[q], F(i + 2 * q), F(i + 2 * q + 1));
       }
-      const float c = score_factor(ka, unit, a.score_log2), lv = __log2f(va), iv = __frcp_rn(va);
+      const float c = unit.of(ka), lv = __log2f(va);
       const float top = fmaf(fmax3(r[0], r[1], fmaxf(r[2], r[3])), c, lv);
       const bool grow = top > m + kSlack;                 // also from m = -inf
       if (__any_sync(0xffffffffu, grow)) {
-        const float alpha = grow ? ex2_approx(m - top) : 1.f;
+        const float half = grow ? half_ex2(m - top) : 1.f, alpha = half * half;
         if (grow) m = top;
-        l *= alpha;
+        l = l * half * half;
         if (u > 0) {                                      // products up to page u - 2 are complete, as its scores are
           if (!(ok = mbar_wait(&sh->o_done[t][(u - 1) & 1], ((u - 1) >> 1) & 1, abort_flag, a.status, kDevTimeoutO))) break;
           tc_fence_after();
@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
           }
         }
       }
-      const float ref = lv - ((m == -INFINITY ? 0.f : m) - kWeightBits);
+      const float lift = lv + faint_exponent(top, m);
+      const float ref = lift - ((m == -INFINITY ? 0.f : m) - kWeightBits);
       const uint64_t c2 = f2_pack(c, c), b2 = f2_pack(ref, ref);
       uint64_t acc[2] = {0, 0};
 #pragma unroll
@@ -361,8 +362,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
       float s[4];
       f2_unpack(acc[0], s[0], s[1]);
       f2_unpack(acc[1], s[2], s[3]);
-      l = fmaf((s[0] + s[1]) + (s[2] + s[3]), iv, l);     // (a quotient by __fdividef is 0 for va above 2^126)
+      l = fmaf((s[0] + s[1]) + (s[2] + s[3]), ex2_approx(kSumBits - lift), l);
     }
+    l *= kSumUnit;
     if (ok && n > 0) ok = mbar_wait(&sh->o_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, a.status, kDevTimeoutO);
     tc_fence_after();
     // ---------------------------------------------------------- result: O / (Q l), or the split's O / Q, m - 7, l

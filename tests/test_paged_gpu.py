@@ -620,3 +620,49 @@ def test_attend_subnormal_rows(fmt, lq):
     for causal in (False, True):
         run_attend(q[:1], (k, v, ka, va), table[:1], [150], [lq], causal)
         run_attend(q[1:], (k, v, ka, va), table[1:], [190], [lq], causal, sm_scale=2.0 ** -85)
+
+
+def run_unlike(q, pages, table, kv, causal, **kw):
+    """run_attend for one sequence whose V scales lie any distance apart. A weight is 2^7 times p_j amax_j / M at least, M the
+    row's largest p amax, and its rounding to fp16 is off by 2^-25 at most where 2^-11 relative is less: in the output by
+    2^-32 M |d_j| / (Q sum p), d_j the code. That is not a part of |v_j| where amax_j is far below M, as the 64-bit
+    evaluation's tolerance has it."""
+    from lingbot_b200 import paged_cache as pc
+    k, v, ka, va = pages
+    out, lse = pc.attend(q.cuda(), pool(pages), table.cuda(), i32([kv]), causal=causal, return_lse=True, **kw)
+    ref, ref_lse, tol = P.attend(q, *pages, table, [kv], [q.shape[1]], causal)
+    row, lq, top = table[0], q.shape[1], P.TOP[v.dtype]
+    amax = P.gather(torch.full_like(v.float(), top).to(v.dtype), va, row, kv, v.dtype)[:, 0, 0]
+    d = P.gather(v, torch.full_like(va, top), row, kv, v.dtype)[:, 0].abs().sum(0)
+    for h in range(q.shape[2]):
+        x = q[0, :, h].double() @ P.gather(k, ka, row, kv, k.dtype)[:, 0].T * 128 ** -0.5
+        if causal:
+            x = x.masked_fill(torch.arange(kv)[None] > kv - lq + torch.arange(lq)[:, None], -torch.inf)
+        p = torch.softmax(x, -1)
+        tol[0, :, h] += 2.0 ** -32 * (p * amax).amax(-1, keepdim=True) * d / top
+    err = (out.cpu().double() - ref).abs()
+    tol = tol + torch.finfo(q.dtype).eps / 2 * ref.abs() * 1.01 + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+    assert bool((err <= tol).all()), (float((err - tol).max()), float((err / tol).max()))
+    assert bool(((lse.cpu().double() - ref_lse).abs() <= 2.0 ** -11 + 2.0 ** -20 * ref_lse.abs()).all())
+
+
+@FORMATS
+@pytest.mark.parametrize("lq", [1, 40, 129], ids=["token", "few", "many"])
+def test_attend_values_of_unlike_pages(fmt, lq):
+    """V scales of one sequence from 2^-40 (a page of zeros) to 2^127, the large ones first, last and between: the small
+    pages' keys count in full in the sum and the log-sum-exp, whatever the order, the splits and the scores."""
+    g = torch.Generator().manual_seed(6)
+    k, v, ka, va = P.make_pages(17, 14, 1, fmt)
+    v.view(torch.int8)[2] = 0
+    table = P.make_table(6, [13], 14)
+    q = torch.randn(1, lq, 2, 128, generator=g).bfloat16()
+    tiny, one, huge = 2.0 ** -40, 1.0, 1.7 * 2.0 ** 126
+    for scales in ([tiny] * 13 + [huge], [huge] + [tiny] * 13, [tiny, huge] * 7, [tiny] * 6 + [one] + [huge] + [tiny] * 6,
+                   [2.0 ** (-40 + 12.5 * i) for i in range(14)], [2.0 ** (122.5 - 12.5 * i) for i in range(14)]):
+        by_place = torch.tensor(scales).bfloat16().float()
+        va = torch.empty(14, 1)
+        va[table[0].long(), 0] = by_place[:13]
+        va[[i for i in range(14) if i not in table[0].tolist()], 0] = by_place[13]
+        for splits in (1, 3, 9):
+            run_unlike(q, (k, v, ka, va), table, 810, True, num_splits=splits)
+        run_unlike(q * 40, (k, v, ka, va), table, 810, False)
