@@ -162,3 +162,52 @@ def device_status(clear=True):
     out = _i32(0)
     call("lbq_device_status", int(bool(clear)), ctypes.byref(out))
     return out.value
+
+
+def _reaches(dims, at, width, zero):
+    """Whether some sum of c * stride over dims (stride, least c, most c) lies nearer than `width` to `at`; with zero False,
+    one whose c are not all 0. Strides far apart, as a tensor's are, leave one or two c to try at each; a case of very many
+    counts as reached."""
+    dims = sorted(dims, reverse=True)
+    below = [(0, 0)]                                             # least and most of the smaller strides' sums
+    for st, lo, hi in reversed(dims):
+        below.append((below[-1][0] + lo * st, below[-1][1] + hi * st))
+    below.reverse()
+    todo = [(0, at, zero)]
+    for _ in range(10000):
+        if not todo:
+            return False
+        i, d, ok = todo.pop()
+        if i == len(dims):
+            if ok and -width < d < width:
+                return True
+            continue
+        st, lo, hi = dims[i]
+        least, most = below[i + 1]
+        lo = max(lo, -((most + width - 1 - d) // st))
+        hi = min(hi, (d + width - 1 - least) // st)
+        todo += [(i + 1, d - c * st, ok or c != 0) for c in range(lo, min(hi, lo + 10000) + 1)]
+    return True
+
+
+def self_overlap(t):
+    """Whether elements of a tensor with unit last stride share memory with one another."""
+    if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+        return True
+    dims = [(st, 1 - n, n - 1) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
+    return t.numel() > 0 and _reaches(dims, 0, t.shape[-1], False)
+
+
+def share_memory(a, b):
+    """Whether two tensors of one type and one last dimension, of unit stride, have elements in common memory; not where
+    their addresses alternate, as those of views of one buffer do."""
+    if not a.numel() or not b.numel():
+        return False
+    size, width = a.element_size(), a.shape[-1] * a.element_size()
+    at, dims = b.data_ptr() - a.data_ptr(), {}
+    for t, sign in ((a, 1), (b, -1)):
+        for n, st in zip(t.shape[:-1], t.stride()[:-1]):
+            if n > 1 and st > 0:
+                lo, hi = dims.get(st * size, (0, 0))
+                dims[st * size] = (lo, hi + n - 1) if sign == 1 else (lo - n + 1, hi)
+    return _reaches([(st, lo, hi) for st, (lo, hi) in dims.items()], at, width, True)

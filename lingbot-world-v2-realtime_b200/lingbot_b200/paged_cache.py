@@ -206,6 +206,10 @@ def window(pages: Pages, page_table, start, length, dtype=torch.bfloat16, lens=N
             if tuple(t.shape[:3]) != (b, length, heads) or t.dtype != dtype:
                 raise ValueError(f"{name} must be {dtype} [{b}, {length}, {heads}, {HEAD_DIM}], got {t.dtype} "
                                  f"{tuple(t.shape)}")
+            if _lib.self_overlap(t):
+                raise ValueError(f"{name} has elements that share memory")
+        if _lib.share_memory(k, v):
+            raise ValueError("k out and v out share memory")
     if b == 0 or length == 0:
         return k, v
     table = _table(page_table, b, dev)
@@ -249,7 +253,7 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
         _check_rows("out", out, dev)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
-        if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+        if _lib.self_overlap(out):
             raise ValueError("out has elements that share memory")
         if (out.data_ptr() != q.data_ptr() or out.stride() != q.stride()) and _overlap(out, q):
             raise ValueError("out overlaps q without being it")

@@ -374,3 +374,42 @@ def test_write_refuses_rope_tables_that_end_before_the_tokens(monkeypatch):
         c.write(0, plan, k, k, rope=r, positions=torch.zeros(2, 101, dtype=torch.int32))
         c.write(0, plan, k, k)
     assert written == [r, r, None, r, None]
+
+
+def _addresses(t):
+    """Element offsets of a tensor, counted from the start of its storage."""
+    at = torch.tensor(t.storage_offset())
+    for n, st in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(n) * st
+    return at.flatten().tolist()
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_overlaps_are_found_exactly(seed):
+    """Random views of one buffer against their lists of addresses: overlaps inside a tensor, and between two."""
+    r = random.Random(seed)
+    buf = torch.zeros(4000, dtype=torch.bfloat16)
+    found = [0, 0, 0, 0]
+    for _ in range(1500):
+        dim = r.choice([1, 2, 8])
+        pair = []
+        for _ in range(2):
+            shape = [r.randint(1, 4) for _ in range(3)] + [dim]
+            nest = [dim * r.randint(1, 3)]
+            nest += [nest[0] * r.randint(1, 4) + r.choice([0, 0, 1])]
+            nest += [nest[1] * r.randint(1, 4) + r.choice([0, 0, 3])]
+            if pair and r.random() < 0.5:
+                nest = list(pair[0].stride()[:3])
+            r.shuffle(nest)
+            pair.append(buf.as_strided(shape, nest + [1], r.randint(0, 400)))
+        for t in pair:
+            want = len(set(_addresses(t))) < t.numel()
+            found[want] += 1
+            assert _lib.self_overlap(t) == want, (t.shape, t.stride())
+        want = not set(_addresses(pair[0])).isdisjoint(_addresses(pair[1]))
+        found[2 + want] += 1
+        assert _lib.share_memory(*pair) == want, [(t.shape, t.stride(), t.storage_offset()) for t in pair]
+    assert min(found) > 100
+    e = buf[:64].view(1, 1, 8, 8).expand(1, 5, 8, 8)
+    assert _lib.self_overlap(e) and not _lib.self_overlap(e[:, :1]) and _lib.share_memory(e, e[:, 2:, 3:5])
+    assert not _lib.share_memory(e[:, :0], e) and not _lib.self_overlap(e[:, :0])

@@ -666,3 +666,23 @@ def test_attend_values_of_unlike_pages(fmt, lq):
         for splits in (1, 3, 9):
             run_unlike(q, (k, v, ka, va), table, 810, True, num_splits=splits)
         run_unlike(q * 40, (k, v, ka, va), table, 810, False)
+
+
+def test_outputs_that_share_memory_are_refused():
+    from lingbot_b200 import paged_cache as pc
+    p = pool(P.make_pages(8, 4, 2, torch.int8))
+    table, lens = i32([[0, 1], [2, 3]]), i32([100, 128])
+    want = pc.window(p, table, 3, 20)
+    buf = torch.zeros(2, 20, 2, 2, 128, dtype=torch.bfloat16, device="cuda")
+    got = pc.window(p, table, 3, 20, out=(buf[:, :, 0], buf[:, :, 1]))           # of one buffer, one after the other
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    k, v = torch.empty_like(want[0]), torch.empty_like(want[1])
+    flat = torch.zeros(40000, dtype=torch.bfloat16, device="cuda")
+    wide = torch.zeros(2, 20, 3, 128, dtype=torch.bfloat16, device="cuda")
+    for out in ((k, k), (k, v[:, :1].expand(v.shape)), (k[:1].expand(k.shape), v), (wide[:, :, :2], wide[:, :, 1:]),
+                (k, flat.as_strided(k.shape, (20 * 128, 128, 128, 1)))):
+        with pytest.raises(ValueError, match="share memory"):
+            pc.window(p, table, 3, 20, out=out)
+    q = torch.randn(2, 3, 4, 128).bfloat16().cuda()
+    with pytest.raises(ValueError, match="share memory"):
+        pc.attend(q, p, table, lens, out=flat.as_strided(q.shape, (512, 256, 128, 1)))
