@@ -106,7 +106,7 @@ def _check_out(name, x, out):
     same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
     if not same and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
         raise ValueError(f"{name} out shares memory with its input without being it")
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+    if _lib.self_overlap(out):
         raise ValueError(f"{name} out has elements that share memory")
 
 
@@ -156,6 +156,8 @@ def apply(x, rope: Rope, positions=None, start=0, inverse=False, out=None, k=Non
         z = k_out
         if h and hk and (y.data_ptr() == k.data_ptr() or z.data_ptr() == x.data_ptr()):
             raise ValueError("out and k_out are swapped: each is written while the other's input is read")
+        if _lib.share_memory(y, z) or _lib.share_memory(y, k) or _lib.share_memory(z, x):
+            raise ValueError("out and k_out share memory with one another or with the other's input")
     if not (h and hk):
         raise ValueError(f"x with {h} heads and k with {hk}: rotate the one that has heads alone")
     if b and l:

@@ -151,3 +151,25 @@ def test_refusals():
         y = x.clone()
         rope.apply(x, t, out=y, k=y, k_out=torch.empty_like(y))
     assert rope.apply(x[:, :0], t).shape == (1, 0, 2, 128)
+
+
+def test_outputs_of_both_tensors_are_their_own_memory():
+    """Q and K of one fused buffer rotate in place; one buffer for both results, or a result over the other's input, is
+    refused."""
+    from lingbot_b200 import rope
+    table = rope.tables(64, 128)
+    buf = torch.randn(2, 9, 5, 128, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+    q, k = buf[:, :, :3], buf[:, :, 3:]
+    want = rope.apply(q, table, k=k)
+    hold = torch.empty(2, 9, 5, 128, dtype=torch.bfloat16, device="cuda")
+    one = torch.empty(2, 9, 3, 128, dtype=torch.bfloat16, device="cuda")
+    flat = torch.empty(20000, dtype=torch.bfloat16, device="cuda")
+    for x, y, out, k_out in ((q, k, one, one[:, :, :2]), (q, k, hold[:, :, :3], hold[:, :, 2:4]), (q, k, one, q[:, :, 1:]),
+                             (q, k, k[:, :, :1].expand(q.shape), one[:, :, :2]), (buf[:, :, :4], buf[:, :, 3:], buf[:, :, :4], buf[:, :, 3:]),
+                             (q, k, flat.as_strided(q.shape, (9 * 256, 256, 64, 1)), one[:, :, :2])):
+        with pytest.raises(ValueError, match="share|swapped"):
+            rope.apply(x, table, k=y, out=out, k_out=k_out)
+    got = rope.apply(q, table, k=k, out=hold[:, :, :3], k_out=hold[:, :, 3:])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    got = rope.apply(q, table, k=k, out=q, k_out=k)
+    assert torch.equal(got[0], want[0]) and torch.equal(buf[:, :, 3:], want[1])
