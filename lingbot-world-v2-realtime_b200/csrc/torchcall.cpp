@@ -58,10 +58,10 @@ int dtype_code(const at::Tensor& t) {
   const auto d = t.scalar_type();
   return d == at::kBFloat16 ? 0 : d == at::kHalf ? 1 : d == at::kFloat ? 2 : -1;
 }
-// [B, L, heads, dim] with unit channel stride on CUDA device `dev`, no gradient wanted.
+// [B, L, heads, dim] with unit channel stride on CUDA device `dev`, no gradient wanted (nor a forward-mode tangent carried).
 bool rows(const at::Tensor& t, int dev) {
   return t.dim() == 4 && t.stride(3) == 1 && t.is_cuda() && t.get_device() == dev && t.numel() > 0 &&
-         !(t.requires_grad() && c10::GradMode::is_enabled()) && t.layout() == at::kStrided;
+         !(t.requires_grad() && c10::GradMode::is_enabled()) && !t._fw_grad(0).defined() && t.layout() == at::kStrided;
 }
 bool ints(const at::Tensor& t, int dev, int64_t n) {
   return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_cuda() && t.get_device() == dev &&

@@ -164,6 +164,15 @@ def device_status(clear=True):
     return out.value
 
 
+def no_gradient(what, *tensors):
+    """Refuses tensors through which a gradient is wanted, backward or forward: the kernels record none."""
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} records no gradient: call it under torch.no_grad()")
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} records no gradient, and its result would carry no tangent: pass the primal")
+
+
 def _reaches(dims, at, width, zero):
     """Whether some sum of c * stride over dims (stride, least c, most c) lies nearer than `width` to `at`; with zero False,
     one whose c are not all 0. Strides far apart, as a tensor's are, leave one or two c to try at each; a case of very many

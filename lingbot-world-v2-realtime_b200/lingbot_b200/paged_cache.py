@@ -129,11 +129,6 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
-def _no_grad():
-    if torch.is_grad_enabled():
-        raise RuntimeError("the paged cache records no gradient: call it under torch.no_grad()")
-
-
 def write(pages: Pages, page_table, start, k, v, lens=None, rope: Rope = None, positions=None):
     """Quantizes new tokens k, v [B, L, heads, 128] (bf16 or fp16) into the pages of tokens start[b] .. start[b] +
     lens[b] (start, lens: int32 [B] tensors or ints; lens None: all L). A page that already holds tokens before `start`
@@ -152,8 +147,7 @@ def write(pages: Pages, page_table, start, k, v, lens=None, rope: Rope = None, p
     if v.shape != k.shape or v.dtype != k.dtype or k.shape[2] != heads:
         raise ValueError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ, or are not of the pages' "
                          f"{heads} heads")
-    if k.requires_grad or v.requires_grad:
-        _no_grad()
+    _lib.no_gradient("the paged cache", k, v)
     b, l = k.shape[:2]
     if b == 0 or l == 0:
         return
@@ -245,8 +239,7 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
     group = hq // heads
     if group * heads != hq or hq == 0:
         raise ValueError(f"q has {hq} heads, not a multiple of the pages' {heads}")
-    if q.requires_grad:
-        _no_grad()
+    _lib.no_gradient("the paged cache", q)
     if out is None:
         out = torch.empty_like(q)
     else:

@@ -124,10 +124,8 @@ def apply(x, rope: Rope, positions=None, start=0, inverse=False, out=None, k=Non
     _check("x", x)
     b, l, h, d = x.shape
     dev = x.device
-    if x.requires_grad or (k is not None and k.requires_grad):
-        if torch.is_grad_enabled():
-            raise RuntimeError("rope.apply records no gradient: call it under torch.no_grad(), and rotate the gradient "
-                               "back with inverse=True")
+    # (the gradient of the rotated tensor is rotated back with inverse=True)
+    _lib.no_gradient("rope.apply", x, *(() if k is None else (k,)))
     start = int(start)
     if not 0 <= start < 1 << 62:
         raise ValueError(f"start {start} must be a non-negative 64-bit position")

@@ -686,3 +686,34 @@ def test_outputs_that_share_memory_are_refused():
     q = torch.randn(2, 3, 4, 128).bfloat16().cuda()
     with pytest.raises(ValueError, match="share memory"):
         pc.attend(q, p, table, lens, out=flat.as_strided(q.shape, (512, 256, 128, 1)))
+
+
+def test_tensors_that_want_a_gradient_are_refused_both_ways():
+    """requires_grad under grad mode, and forward-mode tangents, which grad mode does not switch off: in every argument,
+    through the short path and the long one."""
+    import torch.autograd.forward_ad as fwd
+    from lingbot_b200 import paged_cache as pc, rope
+    p = pool(P.make_pages(8, 4, 2, torch.int8))
+    table, lens, t = i32([[0, 1], [2, 3]]), i32([100, 128]), rope.tables(64, 128)
+    q = torch.randn(2, 3, 2, 128).bfloat16().cuda()
+
+    def calls(x):
+        return [lambda: pc.attend(x, p, table, lens), lambda: pc.attend(x, p, table, lens, out=torch.empty_like(q)),
+                lambda: pc.write(p, table, 0, x, q), lambda: pc.write(p, table, 0, q, x, lens=2),
+                lambda: rope.apply(x, t), lambda: rope.apply(q, t, k=x), lambda: rope.apply(x, t, out=torch.empty_like(q))]
+    before = p.k.clone()
+    for call in calls(q.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+    with fwd.dual_level():
+        dual = fwd.make_dual(q, torch.ones_like(q))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                for call in calls(dual):
+                    with pytest.raises(RuntimeError, match="tangent"):
+                        call()
+        assert torch.equal(pc.attend(fwd.unpack_dual(dual).primal, p, table, lens), pc.attend(q, p, table, lens))
+    assert torch.equal(raw(p.k), raw(before))
+    with torch.no_grad():
+        for call in calls(q.clone().requires_grad_()):
+            call()
