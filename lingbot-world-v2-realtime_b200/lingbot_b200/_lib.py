@@ -201,6 +201,8 @@ def _reaches(dims, at, width, zero):
 
 def self_overlap(t):
     """Whether elements of a tensor with unit last stride share memory with one another."""
+    if t.is_contiguous():
+        return False
     if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
         return True
     dims = [(st, 1 - n, n - 1) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
