@@ -415,8 +415,8 @@ LBQ_API int lbq_page_copy(void* k_pages, float* k_amax, void* v_pages, float* v_
                           int layers, int64_t layer_bytes, int64_t layer_amax, const int32_t* src, const int32_t* dst,
                           int pairs, void* stream);
 
-/* Key splits to give lbq_paged_attn for these shapes (ragged != 0: sequences of unlike lengths, at most max_kv_len), and the
- * scratch bytes of a split count (0 for one). */
+/* Key splits to give lbq_paged_attn for these shapes (ragged != 0: sequences of unlike key lengths, at most max_kv_len, their
+ * mean under about two thirds of it), and the scratch bytes of a split count (0 for one). */
 LBQ_API int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t max_kv_len, int ragged);
 LBQ_API size_t lbq_paged_attn_workspace(int batch, int q_len, int heads, int group, int num_splits);
 

@@ -260,10 +260,10 @@ PyObject* page_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// paged_attn(pool, device, q, table, kv_lens, q_lens or None, causal, sm_scale): out
+// paged_attn(pool, device, q, table, kv_lens, q_lens or None, causal, sm_scale, ragged or None): out
 PyObject* paged_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 8 || !PyTuple_CheckExact(args[0])) Py_RETURN_NONE;
+  if (n != 9 || !PyTuple_CheckExact(args[0])) Py_RETURN_NONE;
   const Pool pool(args[0]);
   const int dev = static_cast<int>(PyLong_AsLong(args[1]));
   const at::Tensor *q = tensor(args[2]), *table = tensor(args[3]);
@@ -281,7 +281,9 @@ PyObject* paged_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (scale == -1.0 && PyErr_Occurred()) return nullptr;
   const int group = int(hq / pool.heads);
   const int64_t longest = kv ? table->size(1) * 64 : kv0;
-  const int splits = f_splits(int(b), int(lq), pool.heads, group, longest, b > 1 && ql != nullptr);
+  const int ragged = args[8] == Py_None ? kv != nullptr : PyObject_IsTrue(args[8]);
+  if (ragged < 0) return nullptr;
+  const int splits = f_splits(int(b), int(lq), pool.heads, group, longest, b > 1 && ragged);
   at::Tensor out = at::empty_like(*q), ws;
   const size_t need = f_workspace(int(b), int(lq), pool.heads, group, splits);
   if (need > 0) ws = at::empty({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));

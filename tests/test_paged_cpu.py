@@ -413,3 +413,19 @@ def test_overlaps_are_found_exactly(seed):
     e = buf[:64].view(1, 1, 8, 8).expand(1, 5, 8, 8)
     assert _lib.self_overlap(e) and not _lib.self_overlap(e[:, :1]) and _lib.share_memory(e, e[:, 2:, 3:5])
     assert not _lib.share_memory(e[:, :0], e) and not _lib.self_overlap(e[:, :0])
+
+
+def test_key_splits_follow_the_key_lengths(monkeypatch):
+    """A plan knows whether its sessions' lengths are unlike, whatever their new tokens; one that takes later values may be."""
+    pool = Tokens(monkeypatch, 30)
+    c = pool.cache
+    seen = []
+    monkeypatch.setattr(paged_cache, "attend", lambda *a, ragged, **kw: seen.append(ragged))
+    a, b, d = c.open(), c.open(), c.open()
+    c.commit(c.plan([a, b, d], [400, 390, 20]))
+    q = torch.zeros(2, 64, 1, 128)
+    for sessions, new in (([a, b], 1), ([a, b], [1, 64]), ([a, d], 1), ([a, d], [1, 64]), ([d], 1), ([a, b, d], [0, 0, 63])):
+        c.attend(0, c.plan(sessions, new), q)
+    c.attend(0, c.plan([a, b], 1, into=c.fixed_plan(2)), q)
+    assert seen == [False, False, True, True, False, False, True]
+    assert 3 * (400 + 390 + 83) > 2 * 3 * 400

@@ -717,3 +717,25 @@ def test_tensors_that_want_a_gradient_are_refused_both_ways():
     with torch.no_grad():
         for call in calls(q.clone().requires_grad_()):
             call()
+
+
+def test_key_splits_follow_the_key_lengths_not_the_padding():
+    """The same splits, so the same bits, with q_lens and without, and on the short path as on the long one; lengths as an
+    int, or said to be alike, take the other rule's."""
+    from lingbot_b200 import _lib, paged_cache as pc
+    n, h, g = 16, 8, 4
+    pages = P.make_pages(21, 16 * 40, h, torch.int8)
+    p = pool(pages)
+    table = torch.arange(n * 40, dtype=torch.int32).view(n, 40).cuda()
+    q = torch.randn(n, 1, h * g, 128, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    alike, unlike = (_lib.load().lbq_paged_attn_splits(n, 1, h, g, 2560, r) for r in (0, 1))
+    assert alike != unlike
+    lens, ones = torch.full((n,), 2560, dtype=torch.int32).cuda(), i32([1] * n)
+    want = {r: pc.attend(q, p, table, lens, num_splits=s) for r, s in ((False, alike), (True, unlike))}
+    assert not torch.equal(want[False], want[True])
+    for kw, r in ((dict(), True), (dict(q_lens=ones), True), (dict(ragged=True), True), (dict(ragged=False), False),
+                  (dict(q_lens=ones, ragged=False), False)):
+        assert torch.equal(pc.attend(q, p, table, lens, **kw), want[r])
+        assert torch.equal(pc.attend(q, p, table, lens, out=torch.empty_like(q), **kw), want[r])
+    assert torch.equal(pc.attend(q, p, table, 2560), want[False])
+    assert torch.equal(pc.attend(q, p, table, 2560, q_lens=ones, out=torch.empty_like(q)), want[False])
