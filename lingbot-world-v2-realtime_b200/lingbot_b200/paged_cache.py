@@ -15,6 +15,7 @@ Two levels:
 from __future__ import annotations
 
 import ctypes
+import heapq
 from array import array
 from dataclasses import dataclass
 
@@ -330,7 +331,7 @@ class PagedCache:
         self.layers = [pages.layer(i) for i in range(pages.k.shape[0])]
         self.num_pages = pages.k.shape[1]
         self.max_pages = int(max_pages)
-        self._free = list(range(self.num_pages - 1, -1, -1))      # ascending ids are taken first
+        self._free = list(range(self.num_pages))                  # a heap: the lowest ids are taken first
         self._refs = [0] * self.num_pages
         self._sessions = {}                                       # id -> [pages, tokens, version, evicted tokens]
         self._next = 0
@@ -358,15 +359,14 @@ class PagedCache:
         self._sessions[session][2] = self._version
 
     def _take(self):
-        page = self._free.pop()
+        page = heapq.heappop(self._free)
         self._refs[page] = 1
         return page
 
     def _drop(self, page):
         self._refs[page] -= 1
         if self._refs[page] == 0:
-            self._free.append(page)
-            self._free.sort(reverse=True)
+            heapq.heappush(self._free, page)
 
     def open(self):
         """A new, empty session."""
@@ -543,7 +543,7 @@ class PagedCache:
                 self._touch(s)
         for s, d in to.items():
             self._refs[d], self._refs[s] = self._refs[s], 0
-        self._free = list(range(self.num_pages - 1, live - 1, -1))
+        self._free = list(range(live, self.num_pages))
         return len(src)
 
 

@@ -429,3 +429,23 @@ def test_key_splits_follow_the_key_lengths(monkeypatch):
     c.attend(0, c.plan([a, b], 1, into=c.fixed_plan(2)), q)
     assert seen == [False, False, True, True, False, False, True]
     assert 3 * (400 + 390 + 83) > 2 * 3 * 400
+
+
+def test_closing_a_long_session_takes_no_time(monkeypatch):
+    """40000 pages freed one by one, into a pool whose free pages stay in order (sorting them all at each took 4 s)."""
+    import time
+    pool = Tokens(monkeypatch, 2, layers=1)
+    shape = (1, 40000, 1, 64, 128)
+    codes = torch.empty(1, dtype=torch.int8).expand(shape)
+    c = paged_cache.PagedCache(paged_cache.Pages(codes, codes, None, None), max_pages=40000)
+    del pool
+    a, b = c.open(), c.open()
+    c.plan([a], 64 * 39990)
+    c.plan([b], 64 * 10)
+    t0 = time.perf_counter()
+    c.close(a)
+    assert time.perf_counter() - t0 < 2
+    assert c.free_pages == 39990 and c.page_ids(b) == list(range(39990, 40000))
+    s = c.open()
+    c.plan([s], 64 * 5)
+    assert c.page_ids(s) == list(range(5))                           # the lowest free ids
