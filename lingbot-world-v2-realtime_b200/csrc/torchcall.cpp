@@ -54,6 +54,8 @@ const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariab
 int64_t integer(PyObject* o, int i) { return PyLong_AsLongLong(PyTuple_GET_ITEM(o, i)); }
 void* address(PyObject* o, int i) { return PyLong_AsVoidPtr(PyTuple_GET_ITEM(o, i)); }
 
+constexpr int64_t kMostSize = int64_t(1) << 28;                          // of any dimension: the entries take 32-bit sizes
+
 int dtype_code(const at::Tensor& t) {
   const auto d = t.scalar_type();
   return d == at::kBFloat16 ? 0 : d == at::kHalf ? 1 : d == at::kFloat ? 2 : -1;
@@ -61,6 +63,7 @@ int dtype_code(const at::Tensor& t) {
 // [B, L, heads, dim] with unit channel stride on CUDA device `dev`, no gradient wanted (nor a forward-mode tangent carried).
 bool rows(const at::Tensor& t, int dev) {
   return t.dim() == 4 && t.stride(3) == 1 && t.is_cuda() && t.get_device() == dev && t.numel() > 0 &&
+         t.size(0) <= kMostSize && t.size(1) <= kMostSize && t.size(2) <= kMostSize &&
          !(t.requires_grad() && c10::GradMode::is_enabled()) && !t._fw_grad(0).defined() && t.layout() == at::kStrided;
 }
 bool ints(const at::Tensor& t, int dev, int64_t n) {
@@ -68,8 +71,8 @@ bool ints(const at::Tensor& t, int dev, int64_t n) {
          (n <= 1 || t.stride(0) == 1);
 }
 bool table_ok(const at::Tensor& t, int dev, int64_t batch) {
-  return t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == batch && t.size(1) > 0 && t.is_cuda() &&
-         t.get_device() == dev && (t.stride(1) == 1 || t.size(1) == 1);
+  return t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == batch && t.size(1) > 0 &&
+         t.size(1) <= kMostSize && t.is_cuda() && t.get_device() == dev && (t.stride(1) == 1 || t.size(1) == 1);
 }
 // A Python int that is not negative and below 2^62 (a count of tokens can be added to it).
 bool whole(PyObject* o, int64_t* v) {
@@ -140,6 +143,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int64_t start;
   if (!positions(args[4], dev, b, l, &pos) || !whole(args[5], &start)) Py_RETURN_NONE;
   const int inverse = PyObject_IsTrue(args[6]);
+  if (inverse < 0) return nullptr;
   PyObject* r = args[2];
   at::Tensor y = at::empty_like(*x), z;
   if (k != nullptr) z = at::empty_like(*k);
@@ -240,7 +244,7 @@ PyObject* page_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (dev != c10::cuda::current_device() || !table || table->dim() != 2) Py_RETURN_NONE;
   const int64_t b = table->size(0);
   const int dt = static_cast<int>(PyLong_AsLong(args[5]));
-  if (b <= 0 || length <= 0 || length > (1 << 28) || !table_ok(*table, dev, b)) Py_RETURN_NONE;
+  if (b <= 0 || length <= 0 || length > kMostSize || b > kMostSize || !table_ok(*table, dev, b)) Py_RETURN_NONE;
   const int32_t *start, *lens = nullptr;
   int64_t start0, ignored;
   if (!count(args[3], dev, b, &start, &start0)) Py_RETURN_NONE;
@@ -270,13 +274,14 @@ PyObject* paged_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (dev != c10::cuda::current_device() || !q || !table || !rows(*q, dev)) Py_RETURN_NONE;
   const int dt = dtype_code(*q);
   const int64_t b = q->size(0), lq = q->size(1), hq = q->size(2);
-  if (dt < 0 || dt > 1 || q->size(3) != 128 || hq % pool.heads || !table_ok(*table, dev, b) || lq > (1 << 28) || hq > (1 << 24))
+  if (dt < 0 || dt > 1 || q->size(3) != 128 || hq % pool.heads || !table_ok(*table, dev, b) || hq > (1 << 24))
     Py_RETURN_NONE;
   const int32_t *kv, *ql = nullptr;
   int64_t kv0, ignored;
   if (!count(args[4], dev, b, &kv, &kv0)) Py_RETURN_NONE;
   if (args[5] != Py_None && (!count(args[5], dev, b, &ql, &ignored) || ql == nullptr)) Py_RETURN_NONE;
   const int causal = PyObject_IsTrue(args[6]);
+  if (causal < 0) return nullptr;
   const double scale = PyFloat_AsDouble(args[7]);
   if (scale == -1.0 && PyErr_Occurred()) return nullptr;
   const int group = int(hq / pool.heads);

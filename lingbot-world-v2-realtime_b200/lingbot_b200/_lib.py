@@ -164,6 +164,12 @@ def device_status(clear=True):
     return out.value
 
 
+def check_sizes(name, t):
+    """The entries take 32-bit sizes, which ctypes would cut (an expanded dimension needs no memory to be longer)."""
+    if any(n > 1 << 28 for n in t.shape):
+        raise ValueError(f"{name}: {tuple(t.shape)} has a dimension of more than 2^28")
+
+
 def no_gradient(what, *tensors):
     """Refuses tensors through which a gradient is wanted, backward or forward: the kernels record none."""
     for t in tensors:

@@ -87,6 +87,7 @@ def _table(t, batch, device):
     if t.dtype is not torch.int32 or t.dim() != 2 or t.device != device:
         raise ValueError(f"page table: an int32 [batch, pages] tensor on {device}, got {t.dtype} {tuple(t.shape)} on "
                          f"{t.device}")
+    _lib.check_sizes("page table", t)
     n, width = t.shape
     row, unit = t.stride()
     if n != batch or width == 0 or (unit != 1 and width > 1):
@@ -117,6 +118,7 @@ def _check_rows(name, x, device):
         raise ValueError(f"{name} must be [B, L, heads, {HEAD_DIM}] with unit channel stride, got {tuple(x.shape)}")
     if x.device != device:
         raise ValueError(f"{name} on {x.device}, pages on {device}")
+    _lib.check_sizes(name, x)
 
 
 def _overlap(a, b):
@@ -191,6 +193,9 @@ def window(pages: Pages, page_table, start, length, dtype=torch.bfloat16, lens=N
         raise TypeError(f"window dtype {dtype}: expected bfloat16 or float16")
     if length < 0:
         raise ValueError(f"length {length} is negative")
+    if length > 1 << 28:
+        raise ValueError(f"length {length} is more than 2^28")
+    _lib.check_sizes("page table", page_table)
     if out is None:
         k = torch.empty((b, length, heads, HEAD_DIM), dtype=dtype, device=dev)
         v = torch.empty_like(k)

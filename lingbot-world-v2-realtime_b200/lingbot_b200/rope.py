@@ -98,6 +98,7 @@ def _check(name, x):
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
     if x.dim() != 4 or x.stride(3) != 1:
         raise ValueError(f"{name} must be [B, L, heads, dim] with unit channel stride, got {tuple(x.shape)}")
+    _lib.check_sizes(name, x)
 
 
 def _check_out(name, x, out):

@@ -739,3 +739,23 @@ def test_key_splits_follow_the_key_lengths_not_the_padding():
         assert torch.equal(pc.attend(q, p, table, lens, out=torch.empty_like(q), **kw), want[r])
     assert torch.equal(pc.attend(q, p, table, 2560), want[False])
     assert torch.equal(pc.attend(q, p, table, 2560, q_lens=ones, out=torch.empty_like(q)), want[False])
+
+
+def test_sizes_that_pass_32_bits_are_refused():
+    """Expanded dimensions of 2^32 + 5, which 32 bits would turn into 5."""
+    from lingbot_b200 import paged_cache as pc, rope
+    p = pool(P.make_pages(8, 4, 2, torch.int8))
+    table, long = i32([[0, 1]]), (1 << 32) + 5
+    k = torch.ones(1, 1, 2, 128, dtype=torch.bfloat16, device="cuda")
+    before = p.k.clone()
+    for call in (lambda: pc.write(p, table, 0, k.expand(1, long, 2, 128), k.expand(1, long, 2, 128)),
+                 lambda: pc.write(p, table, 0, k.expand(1, long, 2, 128), k.expand(1, long, 2, 128), lens=5),
+                 lambda: pc.write(p, table.expand(long, 2), 0, k.expand(long, 1, 2, 128), k.expand(long, 1, 2, 128)),
+                 lambda: pc.attend(k.expand(1, long, 2, 128), p, table, 100),
+                 lambda: pc.attend(k[:, :, :1].expand(1, 1, 2 * long, 128), p, table, 100),
+                 lambda: pc.window(p, table, 0, long),
+                 lambda: pc.window(p, table.expand(long, 2), 0, 5),
+                 lambda: rope.apply(k.expand(1, long, 2, 128), rope.tables(64, 128))):
+        with pytest.raises(ValueError, match="2.28"):
+            call()
+    assert torch.equal(raw(p.k), raw(before))
