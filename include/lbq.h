@@ -366,7 +366,8 @@ LBQ_API int lbq_peer_wait(const uint64_t* peers, int nranks, int rank, int64_t x
  *   table             int32 [batch] rows of `width` page ids (row stride st_b; ids past a sequence's pages are not
  *                     read): token t of sequence b is row t % 64 of page table[b][t / 64]
  * num_pages * heads * 64 stays below 2^31. A page id outside the pool, or a length or start outside the table, is not
- * followed: it sets the device status to 0x305 (the tokens count as masked, or are not written). */
+ * followed: it sets the device status to 0x305 (the tokens count as masked, or are not written). So does a count of new
+ * tokens or queries outside [0, L], which is cut to it. */
 #define LBQ_PAGE_INT8 0
 #define LBQ_PAGE_E4M3 1
 

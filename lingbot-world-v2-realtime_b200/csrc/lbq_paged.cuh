@@ -22,7 +22,7 @@ constexpr float kTinyScale = 5.421010862427522e-20f;   // 2^-64: scales are kept
 constexpr float kMinFactor = 1.1754943508222875e-38f;  // 2^-126
 // The factor of a row's scores of one page: page (its scale) * row (the power of two taken out of the row) * scale (softmax
 // scale * log2 e / Q). Row and scale are multiplied first, raised by 2^64 where they would underflow though a large page
-// brings them back. It never is 0, which times the -inf of a masked score would be NaN (scores stay below 2^17 in magnitude:
+// brings them back. It never is 0, which times the -inf of a masked score would be NaN (scores stay below 2^33 in magnitude:
 // at the smallest factor they are 0 to any precision).
 struct RowFactor {
   float unit, lower;
@@ -72,7 +72,10 @@ __device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, int b, int
     t.kv = t.kv < 0 ? 0 : most;
   }
   t.qn = a.q_lens ? a.q_lens[b] : a.q_len;
-  t.qn = t.qn < 0 ? 0 : (t.qn > a.q_len ? a.q_len : t.qn);
+  if (t.qn < 0 || t.qn > a.q_len) {
+    if (a.status) atomicCAS(a.status, 0, kDevBadPage);
+    t.qn = t.qn < 0 ? 0 : a.q_len;
+  }
   const int first = tile * a.tile_rows / a.group;                        // first and last query token of the tile
   const int last = min((tile * a.tile_rows + a.tile_rows - 1) / a.group, t.qn - 1);
   if (first > last) t.visible = 0;

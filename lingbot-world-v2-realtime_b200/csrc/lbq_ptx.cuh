@@ -34,7 +34,7 @@ enum DeviceStatus : int {
   kDevBadSourceToken = 0x302,    // debug build: quantizer source token below 0
   kDevBadTile = 0x303,           // debug build: key tile outside its code segment
   kDevBadOwner = 0x304,          // debug build: key-range partial outside the owner's receive slot
-  kDevBadPage = 0x305,           // paged cache: page id outside the pool, or a length outside the page table
+  kDevBadPage = 0x305,           // paged cache: page id outside the pool, a length outside the page table, or a count past L
   kDevBadPosition = 0x306,       // rotary: position outside the tables
 };
 

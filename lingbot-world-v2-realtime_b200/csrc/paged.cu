@@ -172,10 +172,10 @@ __device__ __forceinline__ void write_page(const PageWriteArgs& a, const int w, 
   const int t = threadIdx.x, c16 = t & 15, rg = t >> 4;
   const int64_t start = a.start ? a.start[b] : a.start0;
   int n = a.lens ? a.lens[b] : a.len;
-  n = n < 0 ? 0 : (n > a.len ? a.len : n);
-  if (start < 0) {
+  if (start < 0 || n < 0 || n > a.len) {
     if (a.status && t == 0) atomicCAS(a.status, 0, kDevBadPage);
-    return;
+    if (start < 0 || n < 0) return;
+    n = a.len;
   }
   const int off = int(start % kPageTokens);                              // the first touched page's held rows
   const int l0 = int(blockIdx.x >> 1) * kPageTokens - off;               // source row of this page's row 0

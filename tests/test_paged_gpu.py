@@ -759,3 +759,23 @@ def test_sizes_that_pass_32_bits_are_refused():
         with pytest.raises(ValueError, match="2.28"):
             call()
     assert torch.equal(raw(p.k), raw(before))
+
+
+@pytest.mark.parametrize("lq", [3, 90], ids=["few", "many"])
+def test_counts_past_the_given_tokens_are_recorded(lq):
+    """q_lens and a write's lens outside [0, L] are cut to it, and recorded: the mask or the tokens are not what the caller
+    meant. Counts at the ends are not."""
+    from lingbot_b200 import _lib, paged_cache as pc
+    p = pool(P.make_pages(8, 8, 2, torch.int8))
+    table, lens = i32([[0, 1, 4], [2, 3, 5]]), i32([100, 128])
+    q = torch.randn(2, lq, 2, 128, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    for bad, as_if in (([lq + 1, 1], [lq, 1]), ([1, -1], [1, 0])):
+        got = pc.attend(q, p, table, lens, q_lens=i32(bad), causal=True)
+        assert _lib.device_status() == 0x305
+        assert torch.equal(got, pc.attend(q, p, table, lens, q_lens=i32(as_if), causal=True))
+        a, b = (pool(P.make_pages(8, 8, 2, torch.int8)) for _ in range(2))
+        assert _lib.device_status() == 0
+        pc.write(a, table, 10, q, q, lens=i32(bad))
+        assert _lib.device_status() == 0x305
+        pc.write(b, table, 10, q, q, lens=i32(as_if))
+        assert _lib.device_status() == 0 and torch.equal(raw(a.k), raw(b.k)) and torch.equal(a.v_amax, b.v_amax)
