@@ -20,20 +20,12 @@ __device__ __forceinline__ void after_previous_grid() {
 
 constexpr float kTinyScale = 5.421010862427522e-20f;   // 2^-64: scales are kept above it (a written page's are >= 2^-40)
 constexpr float kMinFactor = 1.1754943508222875e-38f;  // 2^-126
-// The factor of a row's scores of one page: page (its scale) * row (the power of two taken out of the row) * scale (softmax
-// scale * log2 e / Q). Row and scale are multiplied first, raised by 2^64 where they would underflow though a large page
-// brings them back. It never is 0, which times the -inf of a masked score would be NaN (scores stay below 2^33 in magnitude:
-// at the smallest factor they are 0 to any precision).
-struct RowFactor {
-  float unit, lower;
-  __device__ __forceinline__ RowFactor() {}
-  __device__ __forceinline__ RowFactor(float row, float scale) {
-    const bool small = row * scale < 7.888609052210118e-31f;             // 2^-100
-    unit = small ? row * 18446744073709551616.f * scale : row * scale;
-    lower = small ? 5.421010862427522e-20f : 1.f;
-  }
-  __device__ __forceinline__ float of(float page) const { return fmaxf(page * unit * lower, kMinFactor); }
-};
+// The factor of a row's scores of one page is page (its scale) * row (the power of two taken out of the row) * scale (softmax
+// scale * log2 e / Q). Row and scale are multiplied first, with 2^6 moved from the page's part to theirs, so that the smallest
+// rows keep 17 bits and the largest do not overflow. It never is 0, which times the -inf of a masked score would be NaN
+// (scores stay below 2^33 in magnitude: at the smallest factor they are 0 to any precision).
+__device__ __forceinline__ float row_factor(float row, float scale) { return fminf(row * (64.f * scale), 3.402823466e38f); }
+__device__ __forceinline__ float score_factor(float page, float row) { return fmaxf(page * (1.f / 64.f) * row, kMinFactor); }
 // The power of two that scales a bf16 query row of largest magnitude `top` (the bits of the fp32 value) to a maximum in
 // [1, 2), and its inverse `up`. With the exponent field e that is 2^(127 - e); 2^(127 - 254) is no normal float: a maximum
 // in [2, 4) there. A row of subnormals, 2^-126 at most, goes up by 2^127; non-finite rows go as they are.
@@ -48,12 +40,12 @@ constexpr float kSlack = 8.f;                    // ... and the running maximum 
 
 // A page whose largest weight lies more than 2^kFaint below 2^kWeightBits adds nothing to o, but may hold most of the sum
 // when its V are that much smaller (weights carry the scale of V, a page of zeros has 2^-40): its weights would underflow
-// before the division by va. The binary exponent that they, and va, are raised by; `top` is the page's and m the row's
-// maximum. (400: the page's part of the sum is 0 then, and masked pages, top = -inf, stay finite.) While sums are taken they
+// before the division by va. The binary exponent that they, and va, are raised by; `far` is the page's maximum less the
+// row's. (400: the page's part of the sum is 0 then, and masked pages, top = -inf, stay finite.) While sums are taken they
 // are scaled by 2^kSumBits, so that 1 / va (2^128 at most) is no subnormal.
 constexpr float kFaint = 100.f;
 constexpr float kSumBits = 8.f, kSumUnit = 1.f / 256.f;
-__device__ __forceinline__ float faint_exponent(float top, float m) { return fminf(fmaxf(m - top - kFaint, 0.f), 400.f); }
+__device__ __forceinline__ float faint_exponent(float far) { return fminf(fmaxf(-far - kFaint, 0.f), 400.f); }
 // 2^(e / 2): l times it twice. 2^e alone can underflow where the maximum moves for a V scale and not for a score.
 __device__ __forceinline__ float half_ex2(float e) { return ex2_approx(0.5f * e); }
 
@@ -65,16 +57,13 @@ struct TileKeys {
 };
 __device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, int b, int tile) {
   TileKeys t;
-  t.kv = a.kv_lens ? a.kv_lens[b] : a.kv_len0;
   const int64_t most = int64_t(a.pt.width) * kPageTokens;
-  if (t.kv < 0 || t.kv > most) {
+  t.kv = a.kv_lens ? a.kv_lens[b] : a.kv_len0;
+  t.qn = a.q_lens ? a.q_lens[b] : a.q_len;               // both loads before anything waits for one
+  if ((t.kv < 0) | (t.kv > most) | (t.qn < 0) | (t.qn > a.q_len)) {
     if (a.status) atomicCAS(a.status, 0, kDevBadPage);
-    t.kv = t.kv < 0 ? 0 : most;
-  }
-  t.qn = a.q_lens ? a.q_lens[b] : a.q_len;
-  if (t.qn < 0 || t.qn > a.q_len) {
-    if (a.status) atomicCAS(a.status, 0, kDevBadPage);
-    t.qn = t.qn < 0 ? 0 : a.q_len;
+    t.kv = t.kv < 0 ? 0 : min(t.kv, most);
+    t.qn = t.qn < 0 ? 0 : min(t.qn, a.q_len);
   }
   const int first = tile * a.tile_rows / a.group;                        // first and last query token of the tile
   const int last = min((tile * a.tile_rows + a.tile_rows - 1) / a.group, t.qn - 1);

@@ -193,17 +193,17 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
   }
 
   uint2 qb[kNT][8];
-  RowFactor unit[kNT][2];                                // per query column
+  float unit[kNT][2];                                    // per query column
   int limit[kNT][2];                                     // last visible key of the split (a table has under 2^24 pages)
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
     const int r = tile * kRows + 8 * t + r0, i = r / a.group, g = r - i * a.group;
     const uint16_t* row = i < tk.qn ? static_cast<const uint16_t*>(a.q) + b * a.sq[0] + i * a.sq[1] + (h * a.group + g) * a.sq[2]
                                     : nullptr;
-    const float u = load_query<kDt>(row, quad, qb[t]);
+    const float u = row_factor(load_query<kDt>(row, quad, qb[t]), a.score_log2);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      unit[t][e] = RowFactor(__shfl_sync(0xffffffffu, u, 8 * quad + 4 * e), a.score_log2);      // column 2 quad + e is row r0 of that lane
+      unit[t][e] = __shfl_sync(0xffffffffu, u, 8 * quad + 4 * e);      // column 2 quad + e is row r0 of that lane
       const int qi = (tile * kRows + 8 * t + 2 * quad + e) / a.group;
       limit[t][e] = qi >= tk.qn ? -1 : int((a.causal ? tk.kv - tk.qn + qi : tk.kv - 1) - int64_t(p0) * kPageTokens);
     }
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
         for (int mt = 1; mt < 4; ++mt) top = fmax3(top, x[t][mt][e], x[t][mt][2 + e]);
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        c[e] = unit[t][e].of(kat);
+        c[e] = score_factor(kat, unit[t][e]);
         top = fmaf(top, c[e], lv);
         half[e] = 1.f;
         if (top > m[t][e] + kSlack) {                    // also from m = -inf
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2)
           m[t][e] = top;
           grow = true;
         }
-        const float lift = lv + faint_exponent(top, m[t][e]);
+        const float lift = lv + faint_exponent(top - m[t][e]);
         is[e] = ex2_approx(kSumBits - lift);
         // a query that has seen no key yet: its exponents are taken against 0 and are -inf
         bb[e] = lift - ((m[t][e] == -INFINITY ? 0.f : m[t][e]) - kWeightBits);

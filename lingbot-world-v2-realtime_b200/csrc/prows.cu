@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
     const int row = tile * kManyTile + t * 128 + rl, qi = row / a.group, head = h * a.group + (row - qi * a.group);
     const bool on = qi < tk.qn;
     const uint16_t* qrow = on ? static_cast<const uint16_t*>(a.q) + b * a.sq[0] + qi * a.sq[1] + head * a.sq[2] : nullptr;
-    const RowFactor unit(stage_query<kDt>(qrow, sQ + t * kQTile, rl), a.score_log2);
+    const float unit = row_factor(stage_query<kDt>(qrow, sQ + t * kQTile, rl), a.score_log2);
     fence_proxy_async_smem();
     mbar_arrive(&sh->q_full);
     const int limit = !on ? -1 : int((a.causal ? tk.kv - tk.qn + qi : tk.kv - 1) - int64_t(p0) * kPageTokens);
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
 #pragma unroll
         for (int q = 0; q < 4; ++q) r[q] = fmax3(r[q], F(i + 2 * q), F(i + 2 * q + 1));
       }
-      const float c = unit.of(ka), lv = __log2f(va);
+      const float c = score_factor(ka, unit), lv = __log2f(va);
       const float top = fmaf(fmax3(r[0], r[1], fmaxf(r[2], r[3])), c, lv);
       const bool grow = top > m + kSlack;                 // also from m = -inf
       if (__any_sync(0xffffffffu, grow)) {
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const PagedA
           }
         }
       }
-      const float lift = lv + faint_exponent(top, m);
+      const float lift = lv + faint_exponent(top - m);
       const float ref = lift - ((m == -INFINITY ? 0.f : m) - kWeightBits);
       const uint64_t c2 = f2_pack(c, c), b2 = f2_pack(ref, ref);
       uint64_t acc[2] = {0, 0};
