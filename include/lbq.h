@@ -363,8 +363,8 @@ LBQ_API int lbq_peer_wait(const uint64_t* peers, int nranks, int rank, int64_t x
  * A page holds 64 tokens of every K/V head:
  *   k_pages, v_pages  [num_pages][heads][64][128] codes, int8 (LBQ_PAGE_INT8) or e4m3 (LBQ_PAGE_E4M3), 128-byte aligned
  *   k_amax, v_amax    f32 [num_pages][heads]: value = code * amax / 127 (int8) or / 448 (e4m3)
- *   table             int32 [batch] rows of `width` page ids (row stride st_b; ids past a sequence's pages are not
- *                     read): token t of sequence b is row t % 64 of page table[b][t / 64]
+ *   table             int32 [batch] rows of `width` page ids (row stride st_b; all `width` may be loaded, but ids past a
+ *                     sequence's pages are not followed): token t of sequence b is row t % 64 of page table[b][t / 64]
  * num_pages * heads * 64 stays below 2^31. A page id outside the pool, or a length or start outside the table, is not
  * followed: it sets the device status to 0x305 (the tokens count as masked, or are not written). So does a count of new
  * tokens or queries outside [0, L], which is cut to it. */
@@ -386,13 +386,14 @@ LBQ_API int lbq_rope(const void* x, int64_t sx_b, int64_t sx_l, int64_t sx_h, vo
                      int dtype, void* stream);
 
 /* Quantizing write of new tokens k, v [B, L, heads, 128] (dtype bf16 or fp16) at tokens start[b] .. start[b] + lens[b]
- * of each sequence (start null: start0, below 2^62, for all; lens null: L). For a page and head that new tokens x enter, a = max(amax
- * of the tokens it holds before start, max finite |x|, 2^-40); its held codes become round(c * a_old / a), the new ones
- * round(x * Q / a) (exact decisions; int8 half to even, e4m3 to nearest); infinities become +-Q and NaN 0. Rows at and
- * past start that get no new token keep their codes. With rope tables (see lbq_rope; rot a multiple of 8, or of 16 for
- * the half layout; 16-byte aligned, row stride a multiple of 4) K is rotated first, at pos or at its token index,
- * with the bits that lbq_rope followed by the plain write gives. No two sequences of one call may share a page that
- * they write. */
+ * of each sequence (start null: start0, below 2^62, for all; lens null: L). For a page and head that new tokens x enter,
+ * a = max(a_old, max finite |x|, 2^-40), a_old the page's stored amax where it holds tokens before start, else 0; its
+ * held codes become round(c * a_old / a), the new ones round(x * Q / a) (exact decisions; int8 half to even, e4m3 to
+ * nearest); infinities become +-Q and NaN 0. Rows at and past start that get no new token keep their codes; a page that
+ * holds earlier tokens keeps its amax when larger tokens at and past start are replaced. With rope tables (see lbq_rope;
+ * rot a multiple of 8, or of 16 for the half layout; 16-byte aligned, row stride a multiple of 4) K is rotated first, at
+ * pos or at its token index, with the bits that lbq_rope followed by the plain write gives. No two sequences of one call
+ * may share a page that they write. */
 LBQ_API int lbq_page_write(const void* k, int64_t sk_b, int64_t sk_l, int64_t sk_h, const void* v, int64_t sv_b,
                            int64_t sv_l, int64_t sv_h, void* k_pages, float* k_amax, void* v_pages, float* v_amax,
                            int64_t num_pages, int heads, int fmt, const int32_t* table, int64_t st_b, int width,
@@ -424,9 +425,10 @@ LBQ_API size_t lbq_paged_attn_workspace(int batch, int q_len, int heads, int gro
 /* Attention of q [B, Lq, heads * group, 128] (bf16 or fp16; query head h uses K/V head h / group) over the cache:
  * softmax(sm_scale q . k) v over the tokens j < kv_lens[b] (null: kv_len0 for all) and, with causal != 0, j <= kv_lens[b]
  * - q_lens[b] + i for query token i (the queries are the sequence's last tokens). q_lens null: Lq. Codes and scales are
- * used as they are; sums are fp32. Rows that see no token, and rows i >= q_lens[b], become 0 (lse -inf). out as q; lse
- * null or f32 [B, Lq, heads * group], natural logarithm. sm_scale <= 0 means 1/sqrt(128). num_splits > 1 splits the
- * keys; workspace as lbq_paged_attn_workspace says, not shared by calls that may overlap. */
+ * used as they are; sums are fp32, and the softmax's weights are rounded to fp16 for their product with V. Rows that see
+ * no token, and rows i >= q_lens[b], become 0 (lse -inf). out as q; lse null or f32 [B, Lq, heads * group], natural
+ * logarithm. sm_scale <= 0 means 1/sqrt(128). num_splits > 1 splits the keys; workspace as lbq_paged_attn_workspace
+ * says, not shared by calls that may overlap. */
 LBQ_API int lbq_paged_attn(const void* q, int64_t sq_b, int64_t sq_l, int64_t sq_h, const void* k_pages,
                            const float* k_amax, const void* v_pages, const float* v_amax, int64_t num_pages, int heads,
                            int fmt, const int32_t* table, int64_t st_b, int width, const int32_t* kv_lens,

@@ -62,7 +62,7 @@ int check_act16(int dtype) {
                                                            : set_error(LBQ_ERR_ARG, "dtype %d is neither bf16 nor fp16", dtype);
 }
 
-// A rotary table and its positions. `step`: the channels that one thread rotates at once; 0: any even `rot`.
+// A rotary table of any even `rot` up to `dim`, and its positions.
 int make_rope(lbq::RopeTable* r, const float* cs, const float* sn, int64_t stride, int64_t rows, int rot, int interleaved,
               const void* pos, int pos64, int64_t sp_b, int64_t sp_l, int dim) {
   if (!cs || !sn) return set_error(LBQ_ERR_ARG, "rope_cos or rope_sin is null");

@@ -72,7 +72,8 @@ __device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, int b, int
   return t;
 }
 
-// Bytes (s0, s1) of r as a pair of fp16 values: int8 through 1024 + (c + 128), exact; e4m3 by the converter.
+// Bytes (s0, s1) of r as a pair of fp16 values: int8 by the magic-number conversion (a byte put into the low mantissa bits of
+// 1024 is 1024 + (c + 128), and the subtraction is exact), e4m3 by the converter.
 template <int kFmt, int kS0, int kS1>
 __device__ __forceinline__ uint32_t widen(uint32_t r) {
   uint32_t d;

@@ -1,9 +1,11 @@
 // Paged 8-bit KV cache, sm_100a: the quantizing write, the read-back of a window, and page copies (layout and
 // formulas in lbq_paged.h).
 //
-// Write. For a page and head that new tokens x enter: a = max(amax of the tokens it already holds, max finite |x|,
-// 2^-40); held codes c become rnd(c * a_old / a) when a grew, new tokens rnd(x * Q / a) (rnd: round half to even for
-// int8, round to nearest for e4m3); infinities become +-Q and NaN 0, so a cache never holds a non-finite value.
+// Write. For a page and head that new tokens x enter: a = max(a_old, max finite |x|, 2^-40), where a_old is the page's stored
+// amax if it holds tokens before the new ones, else 0 (so it keeps the magnitude of tokens that are replaced now: what was
+// rounded to their scale cannot be had back); held codes c become rnd(c * a_old / a) when a grew, new tokens rnd(x * Q / a)
+// (rnd: round half to even for int8, round to nearest for e4m3); infinities become +-Q and NaN 0, so a cache never holds a
+// non-finite value.
 //
 // The codes are those of exact arithmetic, without a division a value. x and a have at most 11 significant bits, a code
 // at most 7, so a quotient V = x Q / a or c a_old / a is either exactly half way between two codes, or off it by at least

@@ -10,7 +10,10 @@
 // query row is first scaled by a power of two to a maximum in [1, 2), which fp16 holds to 2^-25 of the row's maximum.
 // The scale of V rides in the exponent, so the weights that matter are those nearest 2^7 whatever the pages' magnitudes;
 // m moves only when exceeded by more than 2^8, so weights stay below 2^15 and o, l are rescaled rarely. Weights are
-// rounded to fp16 (2^-12 relative down to 2^-21 of the row's largest), l sums them before the rounding.
+// rounded to fp16 for the product (off by 2^-11 relative at most, and by 2^-32 of the row's largest where that is more); l sums
+// them before the rounding. A second product for what the rounding leaves would double this one's work; an output in bf16 (off
+// by 2^-8) hides the rounding, one in fp16 shows it slightly. Where V scales lie further apart than fp32's exponents, see
+// kFaint (lbq_paged.cuh).
 //
 // Bound by memory: 256 bytes of codes a (key, K/V head) against 512 flops a row. The keys are the M side of the products
 // (S^T = C Q^T, O^T = D^T W^T, mma.sync m16n8k16) and the queries the N side: 8 rows fill a tile, a widened fragment serves

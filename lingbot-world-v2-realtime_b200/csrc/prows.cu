@@ -5,6 +5,7 @@
 //       per row taken out; score x = S * c, c = amax_k * 2^e * softmax scale * log2 e / Q one factor a row and page
 //   P = 2^(x + log2 amax_v - m + 7) as fp16 in tensor memory, over S; O += P . D (D the V codes in fp16)
 //   l += sum P / amax_v (fp32, before the rounding);  out = O / (Q l)
+// P in fp16 is off by 2^-11 relative, as in pattn.cu (bf16 would be off by 2^-8, and tf32 has half the rate).
 //
 // Bound by the tensor pipe and by exp2 alike: a page and 256 rows are 1024 clocks of MMA (8192 flops a clock) and 1024
 // clocks of MUFU. CTA = two 128-row query tiles of one K/V head and key split, 512 threads:

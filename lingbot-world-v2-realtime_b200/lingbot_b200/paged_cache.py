@@ -3,8 +3,8 @@
 The reference's cache is one bf16 buffer a layer whose whole window is quantized again for every attention call
 (lingbot/layers/kv_cache.py:11-88, lingbot/layers/sage_preq.py:107-128; here `kv_cache`). In this one a token is
 quantized once, when it is written (int8 or e4m3 codes, one scale per page, head and tensor), attention reads the codes
-as they are (unquantized queries, fp32 sums), and a page table names the pages of a session, so that sessions share a
-prefix, fork, drop their oldest pages and are packed together without touching other sessions.
+as they are (unquantized queries, fp32 sums, softmax weights in fp16), and a page table names the pages of a session, so
+that sessions share a prefix, fork, drop their oldest pages and are packed together without touching other sessions.
 
 Two levels:
   functions over tensors   write, window, attend, copy_pages on a `Pages` pool, a page table and lengths;
@@ -14,7 +14,6 @@ Two levels:
 """
 from __future__ import annotations
 
-import ctypes
 import heapq
 from array import array
 from dataclasses import dataclass
@@ -136,8 +135,8 @@ def write(pages: Pages, page_table, start, k, v, lens=None, rope: Rope = None, p
     """Quantizes new tokens k, v [B, L, heads, 128] (bf16 or fp16) into the pages of tokens start[b] .. start[b] +
     lens[b] (start, lens: int32 [B] tensors or ints; lens None: all L). A page that already holds tokens before `start`
     keeps them: when its largest magnitude grows their codes are rounded to the new scale. Tokens at and past `start`
-    are replaced. With `rope`, K is rotated on the way, by `positions` [B, L] or its token indices, to the same bits as
-    rope.apply followed by a plain write. Two sequences of one call must not write the same page."""
+    are replaced (a page that holds earlier ones keeps its scale, if a replaced token's was larger). With `rope`, K is
+    rotated on the way, by `positions` [B, L] or its token indices, to the same bits as rope.apply followed by a plain write. Two sequences of one call must not write the same page."""
     if rope is None or rope._dev == pages._dev:
         r = _lib.fast().page_write(pages._args, pages._dev, page_table, start, k, v, lens, None if rope is None else rope._args,
                                    positions)
@@ -230,7 +229,7 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
     """Attention of q [B, Lq, heads, 128] (bf16 or fp16; a multiple of the pages' heads, query head h reading K/V head
     h // group) over the cached tokens j < kv_lens[b] (int32 [B] tensor or int) and, with causal, j <= kv_lens[b] -
     q_lens[b] + i: query i is token kv_lens[b] - q_lens[b] + i of its sequence, already written. q_lens (int32 [B]) marks
-    a padded batch. Rows that see no token, and rows past q_lens[b], are 0. Returns out [B, Lq, heads, 128] in q's dtype,
+    a padded batch. sm_scale None (or not above 0) is 128 ** -0.5. Rows that see no token, and rows past q_lens[b], are 0. Returns out [B, Lq, heads, 128] in q's dtype,
     with return_lse also the rows' log-sum-exp f32 [B, Lq, heads] (-inf for those rows). max_kv_len bounds kv_lens where
     the page table is much wider than the longest sequence. ragged says whether the sequences' key lengths are unlike, their
     mean under about two thirds of the longest (None: yes for a kv_lens tensor, whose values the host does not read, no for an
@@ -327,7 +326,9 @@ class Plan:
 
 class PagedCache:
     """Page bookkeeping of many sessions over one pool with layers. The host knows every length and page; the tensors of
-    a `Plan` carry them to the kernels. Not thread-safe; a session is in one plan at a time."""
+    a `Plan` carry them to the kernels. Not thread-safe; a session is in one plan at a time, which ends when the session's
+    tokens or pages change. Pages that close, evict, plan or compact free are handed out at once: calls of one cache belong on
+    one stream, or behind one another by events, so that what still reads a page comes before what writes it next."""
 
     def __init__(self, pages: Pages, max_pages):
         if pages.k.dim() != 5:
