@@ -229,11 +229,11 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
     """Attention of q [B, Lq, heads, 128] (bf16 or fp16; a multiple of the pages' heads, query head h reading K/V head
     h // group) over the cached tokens j < kv_lens[b] (int32 [B] tensor or int) and, with causal, j <= kv_lens[b] -
     q_lens[b] + i: query i is token kv_lens[b] - q_lens[b] + i of its sequence, already written. q_lens (int32 [B]) marks
-    a padded batch. sm_scale None (or not above 0) is 128 ** -0.5. Rows that see no token, and rows past q_lens[b], are 0. Returns out [B, Lq, heads, 128] in q's dtype,
-    with return_lse also the rows' log-sum-exp f32 [B, Lq, heads] (-inf for those rows). max_kv_len bounds kv_lens where
-    the page table is much wider than the longest sequence. ragged says whether the sequences' key lengths are unlike, their
-    mean under about two thirds of the longest (None: yes for a kv_lens tensor, whose values the host does not read, no for an
-    int). Both only choose the number of key splits, which num_splits overrides."""
+    a padded batch. sm_scale None (or not above 0) is 128 ** -0.5. Rows that see no token, and rows past q_lens[b], are 0.
+    Returns out [B, Lq, heads, 128] in q's dtype, with return_lse also the rows' log-sum-exp f32 [B, Lq, heads] (-inf for
+    those rows). max_kv_len bounds kv_lens where the page table is much wider than the longest sequence. ragged says whether
+    the sequences' key lengths are unlike, their mean under about two thirds of the longest (None: yes for a kv_lens tensor,
+    whose values the host does not read, no for an int); it only chooses the number of key splits, which num_splits overrides."""
     if out is None and not return_lse and max_kv_len is None and num_splits is None:
         r = _lib.fast().paged_attn(pages._args, pages._dev, q, page_table, kv_lens, q_lens, causal, float(sm_scale or 0.0),
                                    ragged)
