@@ -375,8 +375,8 @@ LBQ_API int lbq_peer_wait(const uint64_t* peers, int nranks, int rank, int64_t x
  * [B, L, heads, dim] and, in the same launch, of x2 [B, L, heads2, dim] (null with heads2 = 0): (x0, x1) -> (x0 c -
  * x1 s, x0 s + x1 c) for the pairs (2i, 2i + 1) (interleaved != 0) or (i, i + rot / 2). c, s: row pos of the f32 tables
  * [rope_rows][rot / 2] (row stride rope_stride); pos [B, L] int32 or int64 (pos64; element strides sp_b, sp_l), or null
- * for start + l. inverse != 0 turns back, which is also the gradient. dtype 0 bf16, 1 fp16, 2 fp32; dim even, at most
- * 512; rot even. A position outside the tables sets the device status to 0x306 and leaves its token as it is.
+ * for start + l (start below 2^62). inverse != 0 turns back, which is also the gradient. dtype 0 bf16, 1 fp16, 2 fp32;
+ * dim even, at most 512; rot even. A position outside the tables sets the device status to 0x306 and leaves its token as it is.
  * The reference ropes interleaved pairs by fp64 tables of the chunk's own tokens (transformer.py:134-146). */
 LBQ_API int lbq_rope(const void* x, int64_t sx_b, int64_t sx_l, int64_t sx_h, void* y, int64_t sy_b, int64_t sy_l,
                      int64_t sy_h, int heads, const void* x2, int64_t sx2_b, int64_t sx2_l, int64_t sx2_h, void* y2,
@@ -402,8 +402,8 @@ LBQ_API int lbq_page_write(const void* k, int64_t sk_b, int64_t sk_l, int64_t sk
                            int interleaved, const void* pos, int pos64, int64_t sp_b, int64_t sp_l, int dtype,
                            void* stream);
 
-/* Reads tokens start[b] .. start[b] + lens[b] of each sequence back as values k_out, v_out [B, L, heads, 128] (bf16 or
- * fp16); rows past lens[b] become 0. */
+/* Reads tokens start[b] .. start[b] + lens[b] (start, lens as above) of each sequence back as values k_out, v_out
+ * [B, L, heads, 128] (bf16 or fp16); rows past lens[b] become 0. */
 LBQ_API int lbq_page_read(const void* k_pages, const float* k_amax, const void* v_pages, const float* v_amax,
                           int64_t num_pages, int heads, int fmt, const int32_t* table, int64_t st_b, int width,
                           const int32_t* start, int64_t start0, const int32_t* lens, int batch, int len, void* k_out,

@@ -279,12 +279,12 @@ int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t ma
   const int64_t ctas = (rows + tile - 1) / tile * heads * batch;
   const int64_t pages = (max_kv_len + lbq::kPageTokens - 1) / lbq::kPageTokens;
   // Few rows: two CTAs an SM (296 at once), a split keeps at least 4 pages, one for each warp. Many rows: one CTA an SM, at
-  // least 8 pages to pay for the query tiles. Ragged batches (mean length under two thirds of the longest) get more and shorter splits, which balance the long sequences
-  // (measured, us: CTAs before splitting x longest sequence, with 1 / 2 / 4 / 8 splits. 256 x 8192 keys, all alike 84 / 93 / 100;
-  // ragged 74 / 65 / 60 / 62; 512 x 8192 ragged 117 / 107 / 103; 1024 x 4096 ragged 98 / 104 / 113; 128 x 8192 ragged 51 / 41 /
-  // 28 / 32; 64 x 30000 ragged - / 91 / 70 / 48; 96 x 4100 with 3 / 4 / 6 splits, ragged 25 / 22 / 18, all alike 27 / 34). More
-  // CTAs than SMs want splits of 32 pages and more (ragged, 1 / 2 / 4: 192 x 2048 keys 23 / 20 / 22, 480 x 3000 45 / 48 / 49,
-  // 512 x 2048 35 / 39 / 44, 512 x 30000 366 / 330 / 312).
+  // least 8 pages to pay for the query tiles. Ragged batches (mean length under two thirds of the longest) get more and
+  // shorter splits, which balance the long sequences (measured, us: CTAs before splitting x longest sequence, with 1 / 2 / 4 / 8
+  // splits. 256 x 8192 keys, all alike 84 / 93 / 100; ragged 74 / 65 / 60 / 62; 512 x 8192 ragged 117 / 107 / 103; 1024 x 4096
+  // ragged 98 / 104 / 113; 128 x 8192 ragged 51 / 41 / 28 / 32; 64 x 30000 ragged - / 91 / 70 / 48; 96 x 4100 with 3 / 4 / 6
+  // splits, ragged 25 / 22 / 18, all alike 27 / 34). More CTAs than SMs want splits of 32 pages and more (ragged, 1 / 2 / 4:
+  // 192 x 2048 keys 23 / 20 / 22, 480 x 3000 45 / 48 / 49, 512 x 2048 35 / 39 / 44, 512 x 30000 366 / 330 / 312).
   const bool few = tile != lbq::kManyTile;
   int64_t n = (few ? kFewCtas : 148) / ctas;
   if (few && ragged && pages >= 32 && ctas >= 64 && ctas <= 600) {

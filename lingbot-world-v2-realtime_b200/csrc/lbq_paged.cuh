@@ -22,7 +22,7 @@ constexpr float kTinyScale = 5.421010862427522e-20f;   // 2^-64: scales are kept
 constexpr float kMinFactor = 1.1754943508222875e-38f;  // 2^-126
 // The factor of a row's scores of one page is page (its scale) * row (the power of two taken out of the row) * scale (softmax
 // scale * log2 e / Q). Row and scale are multiplied first, with 2^6 moved from the page's part to theirs, so that the smallest
-// rows keep 17 bits and the largest do not overflow. It never is 0, which times the -inf of a masked score would be NaN
+// rows keep 16 bits and the largest do not overflow. It never is 0, which times the -inf of a masked score would be NaN
 // (scores stay below 2^33 in magnitude: at the smallest factor they are 0 to any precision).
 __device__ __forceinline__ float row_factor(float row, float scale) { return fminf(row * (64.f * scale), 3.402823466e38f); }
 __device__ __forceinline__ float score_factor(float page, float row) { return fmaxf(page * (1.f / 64.f) * row, kMinFactor); }

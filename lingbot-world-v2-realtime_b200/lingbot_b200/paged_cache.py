@@ -136,7 +136,8 @@ def write(pages: Pages, page_table, start, k, v, lens=None, rope: Rope = None, p
     lens[b] (start, lens: int32 [B] tensors or ints; lens None: all L). A page that already holds tokens before `start`
     keeps them: when its largest magnitude grows their codes are rounded to the new scale. Tokens at and past `start`
     are replaced (a page that holds earlier ones keeps its scale, if a replaced token's was larger). With `rope`, K is
-    rotated on the way, by `positions` [B, L] or its token indices, to the same bits as rope.apply followed by a plain write. Two sequences of one call must not write the same page."""
+    rotated on the way, by `positions` [B, L] or its token indices, to the same bits as rope.apply followed by a plain write.
+    Two sequences of one call must not write the same page."""
     if rope is None or rope._dev == pages._dev:
         r = _lib.fast().page_write(pages._args, pages._dev, page_table, start, k, v, lens, None if rope is None else rope._args,
                                    positions)
@@ -233,7 +234,8 @@ def attend(q, pages: Pages, page_table, kv_lens, q_lens=None, causal=False, sm_s
     Returns out [B, Lq, heads, 128] in q's dtype, with return_lse also the rows' log-sum-exp f32 [B, Lq, heads] (-inf for
     those rows). max_kv_len bounds kv_lens where the page table is much wider than the longest sequence. ragged says whether
     the sequences' key lengths are unlike, their mean under about two thirds of the longest (None: yes for a kv_lens tensor,
-    whose values the host does not read, no for an int); it only chooses the number of key splits, which num_splits overrides."""
+    whose values the host does not read, no for an int); it only chooses the number of key splits, which num_splits
+    overrides."""
     if out is None and not return_lse and max_kv_len is None and num_splits is None:
         r = _lib.fast().paged_attn(pages._args, pages._dev, q, page_table, kv_lens, q_lens, causal, float(sm_scale or 0.0),
                                    ragged)
