@@ -86,13 +86,17 @@ int finish(cudaError_t e, const char* what) {
 constexpr int64_t kFewRows = 64;
 int attn_tile_rows(int64_t rows) { return rows <= 8 ? 8 : (rows <= kFewRows ? 16 : lbq::kManyTile); }
 
-// Key splits that fit the GPU at once (two CTAs an SM) and are at most 8 are one cluster, which merges them itself: no
-// workspace, no second launch (one token against 1000 keys x 12 heads, 4 splits: 6.9 against 7.5 us). CTAs of several waves
-// are left to be scheduled one by one (256 CTAs of ragged lengths, 2 splits: 65 us, as clusters 78).
+// At most 8 key splits whose CTAs fit the GPU at once as clusters are one cluster a tile, which merges them itself: no
+// workspace, no second launch. Two CTAs an SM, 296, are more than clusters can fill, since one lies in one group of SMs: up to
+// 256 CTAs they fit and gain 0.5 to 1 us, from 280 on some wait for a second wave (alike, one token x 4096 keys, clustered /
+// not: 64 x 4 CTAs 14.1 / 16.7 us, 32 x 8 10.3 / 11.1, 80 x 3 17.9 / 19.5, 56 x 5 17.1 / 15.7, 72 x 4 22.2 / 16.9, 96 x 3 30.1 /
+// 20.6, 36 x 8 17.6 / 11.5). CTAs of several waves are left to be scheduled one by one.
 constexpr int64_t kFewCtas = 2 * 148;
+constexpr int64_t kClusterCtas = 256;
 bool attn_clustered(int64_t rows, int heads, int batch, int splits) {
   const int tile = attn_tile_rows(rows);
-  return tile != lbq::kManyTile && splits > 1 && splits <= 8 && (rows + tile - 1) / tile * heads * batch * splits <= kFewCtas;
+  return tile != lbq::kManyTile && splits > 1 && splits <= 8 &&
+         (rows + tile - 1) / tile * heads * batch * splits <= kClusterCtas;
 }
 
 }  // namespace
@@ -283,7 +287,7 @@ int lbq_paged_attn_splits(int batch, int q_len, int heads, int group, int64_t ma
   // shorter splits, which balance the long sequences (measured, us: CTAs before splitting x longest sequence, with 1 / 2 / 4 / 8
   // splits. 256 x 8192 keys, all alike 84 / 93 / 100; ragged 74 / 65 / 60 / 62; 512 x 8192 ragged 117 / 107 / 103; 1024 x 4096
   // ragged 98 / 104 / 113; 128 x 8192 ragged 51 / 41 / 28 / 32; 64 x 30000 ragged - / 91 / 70 / 48; 96 x 4100 with 3 / 4 / 6
-  // splits, ragged 25 / 22 / 18, all alike 27 / 34). More CTAs than SMs want splits of 32 pages and more (ragged, 1 / 2 / 4:
+  // splits, ragged 24 / 21 / 17, all alike 26 / 38 / 31). More CTAs than SMs want splits of 32 pages and more (ragged, 1 / 2 / 4:
   // 192 x 2048 keys 23 / 20 / 22, 480 x 3000 45 / 48 / 49, 512 x 2048 35 / 39 / 44, 512 x 30000 366 / 330 / 312).
   const bool few = tile != lbq::kManyTile;
   int64_t n = (few ? kFewCtas : 148) / ctas;

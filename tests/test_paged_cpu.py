@@ -449,3 +449,12 @@ def test_closing_a_long_session_takes_no_time(monkeypatch):
     s = c.open()
     c.plan([s], 64 * 5)
     assert c.page_ids(s) == list(range(5))                           # the lowest free ids
+
+
+def test_only_clusters_that_fit_at_once_merge_in_one():
+    """The merge without scratch is for CTAs that run at once as clusters: up to 256 of them, not up to two an SM (on 148 SMs 72
+    tiles of 4 splits took 22.2 us so, 16.9 with a merge launch)."""
+    ws = _lib.load().lbq_paged_attn_workspace
+    for batch, heads, splits, fit in ((8, 8, 4, True), (4, 8, 8, True), (8, 10, 3, True), (8, 9, 4, False), (8, 12, 3, False),
+                                      (4, 9, 8, False), (8, 6, 6, False), (5, 8, 7, False), (7, 8, 5, False), (1, 1, 9, False)):
+        assert (ws(batch, 1, heads, 1, splits) == 0) == fit, (batch, heads, splits)
